@@ -69,6 +69,11 @@ extern "C" {
 #define QG_OUT_F32    1
 #define QG_OUT_S32    2   /* raw INT32 accumulators (INT8 only) */
 #define QG_OUT_F16    3   /* fp16 (dense formats only) */
+#define QG_OUT_MXFP4  4   /* e2m1 codes and their scale atoms (qg_gemm_gated_mxfp4 only) */
+
+/* Activations of the gated products. */
+#define QG_ACT_SILU       0   /* g / (1 + exp(-g)) */
+#define QG_ACT_GELU_TANH  1   /* 0.5 g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) */
 
 /* Workload configuration for a context. Zero fields take the format default. */
 typedef struct qg_cfg {
@@ -295,6 +300,46 @@ QG_API int  qg_gemm_fp8_b128(const void* A, const void* B, const void* sa, const
 QG_API int  qg_gemm_nvfp4(const void* A, const void* sfa, const void* B, const void* sfb,
                           float ga, float gb, void* C, int out_type, int M, int N, int K, void* stream);
 QG_API int  qg_nvfp4_sf_bytes(int rows, int K, uint64_t* bytes);
+
+/* MXFP4 (OCP Microscaling v1.0): 32 consecutive values along K share a
+ * power-of-two scale.  A tensor is two buffers:
+ *   codes   e2m1, two per byte along K (low nibble = even k), [rows, Kp/2] with
+ *           Kp = K rounded up to 32 (the codes past K are zero);
+ *   scales  ue8m0 bytes s (2^(s-127); 255 = NaN) in 512-byte atoms of 128 rows x
+ *           128 K, ordered [row block][K/128]; inside an atom row r's four scales
+ *           are bytes (r%32)*16 + ((r/32)%4)*4 + 0..3.  qg_mxfp4_sf_bytes gives the
+ *           size; bytes of rows and blocks past the tensor are zero, and a caller
+ *           that makes its own must not leave 255 there.
+ * All four buffers of a product are 16-byte aligned.
+ *
+ * qg_quant_mxfp4: X [M, K] of in_type QG_OUT_BF16 / QG_OUT_F16 / QG_OUT_F32, rows
+ * `ldx` elements apart (K contiguous), any K >= 1.  Per block
+ * e = max(floor(log2 max|x|) - 2, -127), q = e2m1(x * 2^-e), nearest, ties to
+ * even, saturating at 6.  A block with a NaN or an infinity becomes NaN.
+ * qg_dequant_mxfp4: the values again, bf16 or f32 (out_type), exact, [M, K]
+ * with K % 32 == 0 (the padded width).
+ * No counterpart in the reference. */
+QG_API int  qg_mxfp4_sf_bytes(int rows, int K, uint64_t* bytes);
+QG_API int  qg_quant_mxfp4(const void* X, int in_type, int64_t ldx, void* Q, void* SF, int M, int K, void* stream);
+QG_API int  qg_dequant_mxfp4(const void* Q, const void* SF, void* Y, int out_type, int M, int K, void* stream);
+
+/* C[m,n] = out( sum_k a[m,k] b[n,k] ) of two MXFP4 tensors A [M,K] and B [N,K]:
+ * tensor cores (tcgen05.mma kind::mxf4), fp32 accumulate; any M and N,
+ * K % 32 == 0; out_type QG_OUT_BF16 or QG_OUT_F32, C row-major [M,N].
+ * No counterpart in the reference. */
+QG_API int  qg_gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, void* C, int out_type,
+                          int M, int N, int K, void* stream);
+
+/* The gated projections of a feed-forward block, in one kernel:
+ *   H[m,n] = out( act(sum_k a[m,k] wg[n,k]) * sum_k a[m,k] wu[n,k] )
+ * of MXFP4 tensors A [M,K], Wg [N,K] and Wu [N,K]; act is QG_ACT_*.  out_type
+ * QG_OUT_BF16 or QG_OUT_F32: H row-major [M,N], SFH ignored.  QG_OUT_MXFP4
+ * (N % 32 == 0): H receives the codes [M, N/2] and SFH the scale atoms of the
+ * fp32 result's conversion, ready to be the A of the down projection.
+ * No counterpart in the reference. */
+QG_API int  qg_gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void* SFG, const void* Wu,
+                                const void* SFU, void* H, void* SFH, int out_type, int act, int M, int N, int K,
+                                void* stream);
 
 /* W4A16 group-128 decode GEMV / skinny GEMM (1 row on the CUDA cores, 2-12
  * rows on warp MMAs, 13-16 rows on tcgen05, more rows in chunks of 16):

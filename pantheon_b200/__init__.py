@@ -30,6 +30,9 @@ from ._lib import (  # noqa: F401
     QG_OUT_F32,
     QG_OUT_S32,
     QG_OUT_F16,
+    QG_OUT_MXFP4,
+    QG_ACT_SILU,
+    QG_ACT_GELU_TANH,
     QG_GEMV_WEIGHTS_CONST,
     QG_GEMV_ACTIVATIONS_CONST,
     QGError,
@@ -46,6 +49,11 @@ from .ops import (  # noqa: F401
     gemm_e4m3,
     gemm_i8,
     gemm_nvfp4,
+    quant_mxfp4,
+    dequant_mxfp4,
+    mxfp4_sf_bytes,
+    gemm_mxfp4,
+    gemm_gated_mxfp4,
     gen_dense,
     gen_nvfp4,
     nvfp4_sf_bytes,
@@ -62,9 +70,11 @@ from .ops import (  # noqa: F401
 __all__ = [
     "LIB_PATH", "BIN_PATH", "DECODE_BIN_PATH", "MMA_BIN_PATH", "QGError", "load_library", "Workload",
     "device_status", "gemm_i8", "gemm_fp8_b128", "gemm_bf16", "gemm_f16", "gemm_tf32", "gemm_f32", "gemm_e4m3", "gen_dense",
-    "gen_fp8", "gemm_nvfp4", "gen_nvfp4", "nvfp4_sf_bytes", "gemv_w4a16", "gemv_w4a16_workspace_bytes",
+    "gen_fp8", "gemm_nvfp4", "gen_nvfp4", "nvfp4_sf_bytes", "quant_mxfp4", "dequant_mxfp4",
+    "mxfp4_sf_bytes", "gemm_mxfp4", "gemm_gated_mxfp4", "gemv_w4a16", "gemv_w4a16_workspace_bytes",
     "gen_w4a16", "gen_i8", "gen_uniform_f32", "gen_normal_f32", "verify_words",
     "QG_FMT_INT8", "QG_FMT_FP8", "QG_FMT_NVFP4", "QG_FMT_W4A16",
     "QG_FMT_BF16", "QG_FMT_FP16", "QG_FMT_TF32", "QG_FMT_E4M3", "QG_FMT_FP32",
-    "QG_OUT_BF16", "QG_OUT_F32", "QG_OUT_S32", "QG_OUT_F16", "QG_GEMV_WEIGHTS_CONST", "QG_GEMV_ACTIVATIONS_CONST",
+    "QG_OUT_BF16", "QG_OUT_F32", "QG_OUT_S32", "QG_OUT_F16", "QG_OUT_MXFP4", "QG_ACT_SILU",
+    "QG_ACT_GELU_TANH", "QG_GEMV_WEIGHTS_CONST", "QG_GEMV_ACTIVATIONS_CONST",
 ]

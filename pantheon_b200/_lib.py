@@ -21,6 +21,8 @@ QG_ERR_DEVICE_TIMEOUT = 1
 QG_FMT_INT8, QG_FMT_FP8, QG_FMT_NVFP4, QG_FMT_W4A16 = 0, 1, 2, 3
 QG_FMT_BF16, QG_FMT_FP16, QG_FMT_TF32, QG_FMT_E4M3, QG_FMT_FP32 = 4, 5, 6, 7, 8
 QG_OUT_BF16, QG_OUT_F32, QG_OUT_S32, QG_OUT_F16 = 0, 1, 2, 3
+QG_OUT_MXFP4 = 4
+QG_ACT_SILU, QG_ACT_GELU_TANH = 0, 1
 QG_GEMV_WEIGHTS_CONST = 1
 QG_GEMV_ACTIVATIONS_CONST = 2
 
@@ -81,6 +83,12 @@ _SIGNATURES = {
     "qg_gemm_nvfp4": (C.c_int, [_V, _V, _V, _V, C.c_float, C.c_float, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
     "qg_nvfp4_sf_bytes": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
     "qg_gen_nvfp4": (C.c_int, [_V, _V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_uint64, C.c_uint32, _V]),
+    "qg_mxfp4_sf_bytes": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
+    "qg_quant_mxfp4": (C.c_int, [_V, C.c_int, C.c_int64, _V, _V, C.c_int, C.c_int, _V]),
+    "qg_dequant_mxfp4": (C.c_int, [_V, _V, _V, C.c_int, C.c_int, C.c_int, _V]),
+    "qg_gemm_mxfp4": (C.c_int, [_V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
+    "qg_gemm_gated_mxfp4": (C.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                      _V]),
     "qg_gemv_w4a16_workspace_bytes": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
     "qg_gemv_w4a16": (C.c_int, [_V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V, C.c_uint64, _V]),
     "qg_gemv_w4a16_ex": (C.c_int, [_V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V, C.c_uint64, C.c_uint,

@@ -69,6 +69,13 @@ int gen_nvfp4(void* A, void* SFA, void* B, void* SFB, float* gscales, void* work
               uint32_t tid0, cudaStream_t s);
 int gemm_nvfp4(const void* A, const void* SFA, const void* B, const void* SFB, float ga, float gb, void* C,
                int out_type, int M, int N, int K, cudaStream_t stream, const LaunchCheck& chk = LaunchCheck{});
+uint64_t mxfp4_sf_bytes(int rows, int K);
+int quant_mxfp4(const void* X, int in_type, int64_t ldx, void* Q, void* SF, int M, int K, cudaStream_t s);
+int dequant_mxfp4(const void* Q, const void* SF, void* Y, int out_type, int M, int K, cudaStream_t s);
+int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, void* C, int out_type, int M, int N,
+               int K, cudaStream_t stream);
+int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void* SFG, const void* Wu, const void* SFU,
+                     void* H, void* SFH, int out_type, int act, int M, int N, int K, cudaStream_t stream);
 int gen_w4a16(void* X, void* W, void* S, void* Z, int M, int N, int K, uint64_t seed, uint32_t tid0, cudaStream_t s);
 uint64_t gemv_w4a16_workspace_bytes(int M, int N, int K, int sm_count);
 // `chk.expect` (when set) is the golden output, compared word for word by the writer of each output.

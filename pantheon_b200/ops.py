@@ -7,11 +7,12 @@ to the sm_100a kernels in libpantheon_qgemm.so; there is no other path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
 
-from ._lib import (QG_GEMV_ACTIVATIONS_CONST, QG_GEMV_WEIGHTS_CONST, QG_FMT_INT8, QG_FMT_BF16, QG_FMT_FP16, QG_FMT_TF32, QG_FMT_E4M3, QG_FMT_FP32, QG_OUT_BF16, QG_OUT_F16,
+from ._lib import (QG_ACT_GELU_TANH, QG_ACT_SILU, QG_OUT_MXFP4, QG_GEMV_ACTIVATIONS_CONST, QG_GEMV_WEIGHTS_CONST, QG_FMT_INT8, QG_FMT_BF16, QG_FMT_FP16, QG_FMT_TF32, QG_FMT_E4M3, QG_FMT_FP32, QG_OUT_BF16, QG_OUT_F16,
                    QG_OUT_F32, QG_OUT_S32, QGCfg, QGMismatch, QGError, check,
                    last_error, load_library)
 
@@ -184,6 +185,124 @@ def gen_nvfp4(M: int, N: int, K: int, seed: int, tid0: int = 0, device="cuda"):
     check("qg_gen_nvfp4", load_library().qg_gen_nvfp4(_ptr(A), _ptr(sfa), _ptr(B), _ptr(sfb), _ptr(g), _ptr(work),
                                                        M, N, K, seed, tid0, _stream(A.device)))
     return A, sfa, B, sfb, g
+
+
+def _on_device(t: torch.Tensor):
+    """A context in which t's device is the current one (a launch goes to the current device)."""
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _require(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, like: torch.Tensor):
+    """A contiguous CUDA tensor of this type and shape on like's device."""
+    _require_cuda(t)
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != like.device:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+_MX_IN_TYPES = {torch.bfloat16: QG_OUT_BF16, torch.float16: QG_OUT_F16, torch.float32: QG_OUT_F32}
+
+
+def mxfp4_sf_bytes(rows: int, K: int) -> int:
+    """Bytes of the scale atoms of an MXFP4 tensor [rows, K]."""
+    if rows <= 0 or K <= 0:
+        raise ValueError(f"mxfp4_sf_bytes: empty shape {rows}x{K}")
+    return -(-rows // 128) * -(-K // 128) * 512
+
+
+def quant_mxfp4(X: torch.Tensor):
+    """X [M, K] (bf16, fp16 or fp32, K contiguous, rows any stride apart) in MXFP4: (codes, scales).
+
+    codes uint8 [M, Kp/2] (Kp = K rounded up to 32, two e2m1 codes per byte, low nibble = even k),
+    scales uint8 ue8m0 in the atom layout (see include/pantheon_qgemm.h).  A block of 32 that holds
+    a NaN or an infinity becomes NaN.  Asynchronous on the current stream.
+    """
+    if not X.is_cuda:
+        raise ValueError("pantheon_b200 kernels take CUDA tensors only (no CPU fallback)")
+    if X.dim() != 2 or X.dtype not in _MX_IN_TYPES:
+        raise ValueError(f"quant_mxfp4: a 2-D bf16, fp16 or fp32 tensor, got {X.dtype} {list(X.shape)}")
+    M, K = X.shape
+    if K > 1 and X.stride(1) != 1:
+        raise ValueError("quant_mxfp4: the last dimension must be contiguous")
+    if M > 1 and X.stride(0) < K:
+        raise ValueError(f"quant_mxfp4: rows must not overlap (row stride {X.stride(0)} < K={K})")
+    sf = torch.empty((mxfp4_sf_bytes(M, K),), dtype=torch.uint8, device=X.device)
+    q = torch.empty((M, (K + 31) // 32 * 16), dtype=torch.uint8, device=X.device)
+    with _on_device(X):
+        check("qg_quant_mxfp4", load_library().qg_quant_mxfp4(_ptr(X), _MX_IN_TYPES[X.dtype], X.stride(0) if M > 1 else K,
+                                                               _ptr(q), _ptr(sf), M, K, _stream(X.device)))
+    return q, sf
+
+
+def _mx_operand(name: str, Q: torch.Tensor, SF: torch.Tensor, like: torch.Tensor):
+    """(rows, K) of an MXFP4 operand."""
+    if Q.dim() != 2:
+        raise ValueError(f"{name}: codes must be 2-D, got {list(Q.shape)}")
+    rows, K = Q.shape[0], 2 * Q.shape[1]
+    _require(name, Q, torch.uint8, (rows, K // 2), like)
+    _require(f"{name}'s scales", SF, torch.uint8, (mxfp4_sf_bytes(rows, K),), like)
+    return rows, K
+
+
+def dequant_mxfp4(Q: torch.Tensor, SF: torch.Tensor, out_type: int = QG_OUT_BF16) -> torch.Tensor:
+    """The values an MXFP4 tensor stands for, [M, K] bf16 or fp32 (both exact)."""
+    M, K = _mx_operand("dequant_mxfp4: Q", Q, SF, Q)
+    if out_type not in (QG_OUT_BF16, QG_OUT_F32):
+        raise ValueError(f"dequant_mxfp4: out_type {out_type} (bf16 or f32)")
+    out = torch.empty((M, K), dtype=_OUT_DTYPES[out_type], device=Q.device)
+    with _on_device(Q):
+        check("qg_dequant_mxfp4", load_library().qg_dequant_mxfp4(_ptr(Q), _ptr(SF), _ptr(out), out_type, M, K,
+                                                                   _stream(Q.device)))
+    return out
+
+
+def gemm_mxfp4(A: torch.Tensor, sfa: torch.Tensor, B: torch.Tensor, sfb: torch.Tensor, out_type: int = QG_OUT_BF16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """C = A @ B^T of MXFP4 operands A [M, K/2], B [N, K/2] (codes) with their scales: bf16 or fp32 [M, N].
+
+    fp32 accumulation on the tensor cores; any M and N, K % 32 == 0 (what quant_mxfp4 gives).
+    """
+    M, K = _mx_operand("gemm_mxfp4: A", A, sfa, A)
+    N, K2 = _mx_operand("gemm_mxfp4: B", B, sfb, A)
+    if K != K2:
+        raise ValueError(f"K mismatch {K} vs {K2}")
+    if out_type not in (QG_OUT_BF16, QG_OUT_F32):
+        raise ValueError(f"gemm_mxfp4: out_type {out_type} (bf16 or f32)")
+    if out is None:
+        out = torch.empty((M, N), dtype=_OUT_DTYPES[out_type], device=A.device)
+    else:
+        _require("gemm_mxfp4: out", out, _OUT_DTYPES[out_type], (M, N), A)
+    with _on_device(A):
+        check("qg_gemm_mxfp4", load_library().qg_gemm_mxfp4(_ptr(A), _ptr(sfa), _ptr(B), _ptr(sfb), _ptr(out), out_type,
+                                                             M, N, K, _stream(A.device)))
+    return out
+
+
+def gemm_gated_mxfp4(A: torch.Tensor, sfa: torch.Tensor, Wg: torch.Tensor, sfg: torch.Tensor, Wu: torch.Tensor,
+                     sfu: torch.Tensor, act: int = QG_ACT_SILU, out_type: int = QG_OUT_BF16):
+    """H = act(A @ Wg^T) * (A @ Wu^T) of MXFP4 operands A [M, K/2], Wg and Wu [N, K/2], in one kernel.
+
+    out_type QG_OUT_BF16 or QG_OUT_F32 gives H [M, N]; QG_OUT_MXFP4 (N % 32 == 0) gives (codes,
+    scales), the A operand of the down projection.
+    """
+    M, K = _mx_operand("gemm_gated_mxfp4: A", A, sfa, A)
+    N, K2 = _mx_operand("gemm_gated_mxfp4: Wg", Wg, sfg, A)
+    if _mx_operand("gemm_gated_mxfp4: Wu", Wu, sfu, A) != (N, K2) or K != K2:
+        raise ValueError(f"gemm_gated_mxfp4: A {list(A.shape)}, Wg {list(Wg.shape)} and Wu {list(Wu.shape)} do not match")
+    sfh = None
+    if out_type == QG_OUT_MXFP4:
+        if N % 32:
+            raise ValueError(f"gemm_gated_mxfp4: N={N} must be a multiple of 32 for an MXFP4 result")
+        out = torch.empty((M, N // 2), dtype=torch.uint8, device=A.device)
+        sfh = torch.empty((mxfp4_sf_bytes(M, N),), dtype=torch.uint8, device=A.device)
+    elif out_type in (QG_OUT_BF16, QG_OUT_F32):
+        out = torch.empty((M, N), dtype=_OUT_DTYPES[out_type], device=A.device)
+    else:
+        raise ValueError(f"gemm_gated_mxfp4: out_type {out_type} (bf16, f32 or mxfp4)")
+    with _on_device(A):
+        check("qg_gemm_gated_mxfp4",
+              load_library().qg_gemm_gated_mxfp4(_ptr(A), _ptr(sfa), _ptr(Wg), _ptr(sfg), _ptr(Wu), _ptr(sfu), _ptr(out),
+                                                 _ptr(sfh), out_type, act, M, N, K, _stream(A.device)))
+    return (out, sfh) if out_type == QG_OUT_MXFP4 else out
 
 
 def gemv_w4a16_workspace_bytes(M: int, N: int, K: int) -> int:
