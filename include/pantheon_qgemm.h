@@ -341,6 +341,34 @@ QG_API int  qg_gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, 
                                 const void* SFU, void* H, void* SFH, int out_type, int act, int M, int N, int K,
                                 void* stream);
 
+/* The gated projections of a feed-forward block in bf16 or fp16, in one kernel:
+ *   G = X Wg^T, U = X Wu^T, H[m,n] = act(G[m,n]) * U[m,n]
+ * X [M,K], Wg and Wu [N,K], H [M,N], all of the one type, row-major, 16-byte
+ * aligned; N % 8 == 0, K % 8 == 0; fp32 accumulate, H from the unrounded sums.
+ * G and U, both or neither, are kept [M,N] (rounded to the type) for the backward
+ * pass.  Outputs must not overlap operands.
+ * No counterpart in the reference. */
+QG_API int  qg_gemm_gated_bf16(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, int act,
+                               int M, int N, int K, void* stream);
+QG_API int  qg_gemm_gated_f16(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, int act,
+                              int M, int N, int K, void* stream);
+
+/* The backward pass, from dH [M,N] and what the forward pass read and kept:
+ *   dG = dH * U * act'(G), dU = dH * act(G)        (rounded to the type)
+ *   dX = dG Wg + dU Wu [M,K],  dWg = dG^T X, dWu = dU^T X [N,K]
+ * fp32 accumulate, results of the operands' type (written, not added to).  dX, or
+ * dWg and dWu together, may be null: not computed.  `workspace`
+ * (qg_gemm_gated_backward_workspace_bytes, 16-byte aligned, any contents) holds
+ * dG and dU; calls that share one must not overlap on the GPU.
+ * No counterpart in the reference. */
+QG_API int  qg_gemm_gated_backward_workspace_bytes(int M, int N, uint64_t* bytes);
+QG_API int  qg_gemm_gated_bf16_backward(const void* dH, const void* X, const void* Wg, const void* Wu, const void* G,
+                                        const void* U, void* dX, void* dWg, void* dWu, int act, int M, int N, int K,
+                                        void* workspace, uint64_t workspace_bytes, void* stream);
+QG_API int  qg_gemm_gated_f16_backward(const void* dH, const void* X, const void* Wg, const void* Wu, const void* G,
+                                       const void* U, void* dX, void* dWg, void* dWu, int act, int M, int N, int K,
+                                       void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* W4A16 group-128 decode GEMV / skinny GEMM (1 row on the CUDA cores, 2-12
  * rows on warp MMAs, 13-16 rows on tcgen05, more rows in chunks of 16):
  *   Y[m,n] = sum_k X[m,k] * (q[k,n] - Z[k/128,n]) * S[k/128,n],  q = u - 8

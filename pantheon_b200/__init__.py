@@ -54,6 +54,11 @@ from .ops import (  # noqa: F401
     mxfp4_sf_bytes,
     gemm_mxfp4,
     gemm_gated_mxfp4,
+    gemm_gated_bf16,
+    gemm_gated_f16,
+    gemm_gated_bf16_backward,
+    gemm_gated_f16_backward,
+    gemm_gated_backward_workspace_bytes,
     gen_dense,
     gen_nvfp4,
     nvfp4_sf_bytes,
@@ -71,7 +76,8 @@ __all__ = [
     "LIB_PATH", "BIN_PATH", "DECODE_BIN_PATH", "MMA_BIN_PATH", "QGError", "load_library", "Workload",
     "device_status", "gemm_i8", "gemm_fp8_b128", "gemm_bf16", "gemm_f16", "gemm_tf32", "gemm_f32", "gemm_e4m3", "gen_dense",
     "gen_fp8", "gemm_nvfp4", "gen_nvfp4", "nvfp4_sf_bytes", "quant_mxfp4", "dequant_mxfp4",
-    "mxfp4_sf_bytes", "gemm_mxfp4", "gemm_gated_mxfp4", "gemv_w4a16", "gemv_w4a16_workspace_bytes",
+    "mxfp4_sf_bytes", "gemm_mxfp4", "gemm_gated_mxfp4", "gemm_gated_bf16", "gemm_gated_f16",
+    "gemm_gated_bf16_backward", "gemm_gated_f16_backward", "gemm_gated_backward_workspace_bytes", "gemv_w4a16", "gemv_w4a16_workspace_bytes",
     "gen_w4a16", "gen_i8", "gen_uniform_f32", "gen_normal_f32", "verify_words",
     "QG_FMT_INT8", "QG_FMT_FP8", "QG_FMT_NVFP4", "QG_FMT_W4A16",
     "QG_FMT_BF16", "QG_FMT_FP16", "QG_FMT_TF32", "QG_FMT_E4M3", "QG_FMT_FP32",

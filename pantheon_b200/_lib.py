@@ -89,6 +89,13 @@ _SIGNATURES = {
     "qg_gemm_mxfp4": (C.c_int, [_V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
     "qg_gemm_gated_mxfp4": (C.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                       _V]),
+    "qg_gemm_gated_bf16": (C.c_int, [_V, _V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
+    "qg_gemm_gated_f16": (C.c_int, [_V, _V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
+    "qg_gemm_gated_backward_workspace_bytes": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
+    "qg_gemm_gated_bf16_backward": (C.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int,
+                                              _V, C.c_uint64, _V]),
+    "qg_gemm_gated_f16_backward": (C.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int,
+                                             _V, C.c_uint64, _V]),
     "qg_gemv_w4a16_workspace_bytes": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
     "qg_gemv_w4a16": (C.c_int, [_V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V, C.c_uint64, _V]),
     "qg_gemv_w4a16_ex": (C.c_int, [_V, _V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V, C.c_uint64, C.c_uint,

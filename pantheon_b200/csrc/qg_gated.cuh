@@ -13,25 +13,37 @@
 
 namespace qg {
 
-// The logistic's argument of activation ACT.
+// The logistic's argument of activation ACT: g, or 2 sqrt(2/pi) (1 + 0.044715 g^2) g.
 template <int ACT>
 __device__ __forceinline__ float gate_arg(float g) {
     if constexpr (ACT == QG_ACT_SILU) return g;
-    else return g * fmaf(0.0713548162726f, g * g, 1.59576912161f);   // 2 sqrt(2/pi) (1 + 0.044715 g^2) g
+    else return g * fmaf(0.0713548162726f, g * g, 1.59576912161f);
 }
 
 // FAST: the hardware's 2^x and reciprocal, a few units in the last place of
-// fp32, for results that are rounded to 16 bits or fewer.  At y = -88 and below
-// exp(-y) passes the largest fp32 and p is 0, its limit.
+// fp32, for results that are rounded to 16 bits or fewer.  exp(-y) reaches
+// infinity at y = -88.7 and the quotient then is 0 (from 2^126 on with FAST,
+// y = -87.3, where it is below 1.2e-38).
 template <bool FAST>
 __device__ __forceinline__ float logistic(float y) {
-    if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(fminf(-y, 87.0f)));
+    if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(-y));
     else return 1.0f / (1.0f + expf(-y));
 }
 
 template <int ACT, bool FAST>
 __device__ __forceinline__ float gated(float g, float u) {
     return g * logistic<FAST>(gate_arg<ACT>(g)) * u;
+}
+
+// act(g) and its slope.  p (1 - p) is 0 in fp32 from |g| = 30 on, where g^2
+// must not overflow against it: the bend's argument is cut off there.
+template <int ACT>
+__device__ __forceinline__ void gate_slope(float g, float& a, float& s) {
+    const float p = logistic<true>(gate_arg<ACT>(g));
+    const float c = fminf(fmaxf(g, -30.0f), 30.0f);
+    const float dy = ACT == QG_ACT_SILU ? 1.0f : fmaf(3.0f * 0.0713548162726f, c * c, 1.59576912161f);
+    a = g * p;
+    s = fmaf(c * p * (1.0f - p), dy, p);
 }
 
 } // namespace qg

@@ -305,6 +305,84 @@ def gemm_gated_mxfp4(A: torch.Tensor, sfa: torch.Tensor, Wg: torch.Tensor, sfg: 
     return (out, sfh) if out_type == QG_OUT_MXFP4 else out
 
 
+def _gated_shape(entry: str, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, dtype: torch.dtype):
+    if X.dim() != 2 or Wg.dim() != 2:
+        raise ValueError(f"{entry}: X and Wg must be 2-D")
+    M, K = X.shape
+    N = Wg.shape[0]
+    _require(f"{entry}: X", X, dtype, (M, K), X)
+    _require(f"{entry}: Wg", Wg, dtype, (N, K), X)
+    _require(f"{entry}: Wu", Wu, dtype, (N, K), X)
+    return M, N, K
+
+
+def _gemm_gated(entry: str, dtype: torch.dtype, X, Wg, Wu, act, keep):
+    M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
+    out = [torch.empty((M, N), dtype=dtype, device=X.device) for _ in range(3 if keep else 1)]
+    with _on_device(X):
+        check(entry, getattr(load_library(), entry)(_ptr(X), _ptr(Wg), _ptr(Wu), _ptr(out[0]),
+                                                    _ptr(out[1]) if keep else None, _ptr(out[2]) if keep else None,
+                                                    act, M, N, K, _stream(X.device)))
+    return tuple(out) if keep else out[0]
+
+
+def _gemm_gated_backward(entry: str, dtype: torch.dtype, dH, X, Wg, Wu, G, U, act, need_dx, need_dw, workspace):
+    M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
+    for name, t in (("dH", dH), ("G", G), ("U", U)):
+        _require(f"{entry}: {name}", t, dtype, (M, N), X)
+    dX = torch.empty((M, K), dtype=dtype, device=X.device) if need_dx else None
+    dWg = torch.empty((N, K), dtype=dtype, device=X.device) if need_dw else None
+    dWu = torch.empty((N, K), dtype=dtype, device=X.device) if need_dw else None
+    if workspace is None:
+        workspace = torch.empty((4 * M * N,), dtype=torch.uint8, device=X.device)
+    else:
+        _require(f"{entry}: workspace", workspace, torch.uint8, tuple(workspace.shape), X)
+    with _on_device(X):
+        check(entry, getattr(load_library(), entry)(_ptr(dH), _ptr(X), _ptr(Wg), _ptr(Wu), _ptr(G), _ptr(U), _ptr(dX),
+                                                    _ptr(dWg), _ptr(dWu), act, M, N, K, _ptr(workspace),
+                                                    workspace.numel(), _stream(X.device)))
+    return dX, dWg, dWu
+
+
+def gemm_gated_bf16(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, act: int = QG_ACT_SILU, keep: bool = False):
+    """H = act(X @ Wg^T) * (X @ Wu^T) in one kernel: X bf16 [M,K], Wg and Wu bf16 [N,K], H bf16 [M,N].
+
+    keep=True returns (H, G, U) with the two projections rounded to bf16, for
+    gemm_gated_bf16_backward.  N % 8 == 0, K % 8 == 0.
+    """
+    return _gemm_gated("qg_gemm_gated_bf16", torch.bfloat16, X, Wg, Wu, act, keep)
+
+
+def gemm_gated_f16(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, act: int = QG_ACT_SILU, keep: bool = False):
+    """gemm_gated_bf16 with fp16 operands and results."""
+    return _gemm_gated("qg_gemm_gated_f16", torch.float16, X, Wg, Wu, act, keep)
+
+
+def gemm_gated_backward_workspace_bytes(M: int, N: int) -> int:
+    b = C.c_uint64()
+    check("qg_gemm_gated_backward_workspace_bytes",
+          load_library().qg_gemm_gated_backward_workspace_bytes(M, N, C.byref(b)))
+    return b.value
+
+
+def gemm_gated_bf16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, G: torch.Tensor,
+                             U: torch.Tensor, act: int = QG_ACT_SILU, need_dx: bool = True, need_dw: bool = True,
+                             workspace: torch.Tensor | None = None):
+    """Gradients (dX, dWg, dWu) of gemm_gated_bf16 from dH [M,N] and the G, U it kept; a gradient
+    that is not needed is None.  dG and dU are rounded to bf16 on the way.  `workspace` (uint8,
+    gemm_gated_backward_workspace_bytes) is allocated when not given."""
+    return _gemm_gated_backward("qg_gemm_gated_bf16_backward", torch.bfloat16, dH, X, Wg, Wu, G, U, act, need_dx,
+                                need_dw, workspace)
+
+
+def gemm_gated_f16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, G: torch.Tensor,
+                            U: torch.Tensor, act: int = QG_ACT_SILU, need_dx: bool = True, need_dw: bool = True,
+                            workspace: torch.Tensor | None = None):
+    """gemm_gated_bf16_backward in fp16 (values past 65504 become infinities: scale dH as usual)."""
+    return _gemm_gated_backward("qg_gemm_gated_f16_backward", torch.float16, dH, X, Wg, Wu, G, U, act, need_dx,
+                                need_dw, workspace)
+
+
 def gemv_w4a16_workspace_bytes(M: int, N: int, K: int) -> int:
     b = C.c_uint64()
     check("qg_gemv_w4a16_workspace_bytes", load_library().qg_gemv_w4a16_workspace_bytes(M, N, K, C.byref(b)))

@@ -95,3 +95,44 @@ def test_reference_rounds_to_the_nearest_level_with_ties_to_even():
     assert list(code[0, :12]) == [7, 0, 2, 2, 4, 4, 6, 6, 8, 15, 1, 0]
     q, sf = R.pack(code, byte)
     assert list(R.decode(q, sf)[0, :4]) == [6.0, 0.0, 1.0, 1.0]
+
+
+@pytest.mark.parametrize("name", ["qg_gemm_gated_bf16", "qg_gemm_gated_f16"])
+def test_gated_dense_refusals(qglib, name):
+    f = getattr(qglib, name)
+    _refused(f(P, P, None, P, None, None, 0, 4, 8, 8, None), "null")
+    _refused(f(P, P, P, None, None, None, 0, 4, 8, 8, None), "null")
+    _refused(f(P, P, P, P, P, None, 0, 4, 8, 8, None), "together")
+    _refused(f(P, P, P, P, None, None, 2, 4, 8, 8, None), "activation")
+    _refused(f(P, P, P, P, None, None, 0, 0, 8, 8, None), "empty")
+    _refused(f(P, P, P, P, None, None, 0, 4, 12, 8, None), "multiples of 8")
+    _refused(f(P, P, P, P, None, None, 0, 4, 8, 12, None), "multiples of 8")
+    _refused(f(P, P + 8, P, P, None, None, 0, 4, 8, 8, None), "aligned")
+    _refused(f(P, P, P, P + 2, None, None, 0, 4, 8, 8, None), "aligned")
+    _refused(f(P, P, P, P, None, None, 0, 1 << 30, 8, 8, None), "too large")
+
+
+@pytest.mark.parametrize("name", ["qg_gemm_gated_bf16_backward", "qg_gemm_gated_f16_backward"])
+def test_gated_backward_refusals(qglib, name):
+    f = getattr(qglib, name)
+    big = 1 << 30
+    _refused(f(None, P, P, P, P, P, P, P, P, 0, 4, 8, 8, P, big, None), "null")
+    _refused(f(P, P, P, P, P, None, P, P, P, 0, 4, 8, 8, P, big, None), "null")
+    _refused(f(P, P, P, P, P, P, P, P, None, 0, 4, 8, 8, P, big, None), "together")
+    _refused(f(P, P, P, P, P, P, None, None, None, 0, 4, 8, 8, P, big, None), "no gradient")
+    _refused(f(P, P, P, P, P, P, P, P, P, -1, 4, 8, 8, P, big, None), "activation")
+    _refused(f(P, P, P, P, P, P, P, P, P, 0, 4, 8, 20, P, big, None), "multiples of 8")
+    _refused(f(P, P, P, P, P, P, P, P, P, 0, 4, 8, 8, None, big, None), "workspace")
+    b = C.c_uint64()
+    assert qglib.qg_gemm_gated_backward_workspace_bytes(4, 8, C.byref(b)) == 0 and b.value >= 4 * 4 * 8
+    _refused(f(P, P, P, P, P, P, P, P, P, 0, 4, 8, 8, P, b.value - 1, None), "workspace")
+    _refused(f(P, P, P, P, P, P, P, P, P, 0, 4, 8, 8, P + 8, big, None), "aligned")
+    _refused(f(P, P, P, P, P, P, P + 8, P, P, 0, 4, 8, 8, P, big, None), "aligned")
+
+
+def test_gated_dense_refuses_cpu_tensors(qglib):
+    x, w = torch.zeros((4, 8), dtype=torch.bfloat16), torch.zeros((8, 8), dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        pb.gemm_gated_bf16(x, w, w)
+    with pytest.raises(ValueError):
+        pb.gemm_gated_bf16_backward(x, x, w, w, x, x)
