@@ -76,6 +76,11 @@ int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, v
                int K, cudaStream_t stream);
 int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void* SFG, const void* Wu, const void* SFU,
                      void* H, void* SFH, int out_type, int act, int M, int N, int K, cudaStream_t stream);
+namespace mx {
+// Either product for few rows of A (qg_gemm_mxfp4_rows.cu); act < 0 is the plain one.  Arguments are checked by the caller.
+int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,
+              void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream);
+}
 int gen_w4a16(void* X, void* W, void* S, void* Z, int M, int N, int K, uint64_t seed, uint32_t tid0, cudaStream_t s);
 uint64_t gemv_w4a16_workspace_bytes(int M, int N, int K, int sm_count);
 // `chk.expect` (when set) is the golden output, compared word for word by the writer of each output.

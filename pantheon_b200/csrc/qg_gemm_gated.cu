@@ -26,6 +26,7 @@
 #include "qg_common.cuh"
 #include "qg_formats.cuh"
 #include "qg_gated.cuh"
+#include "qg_launch.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -131,7 +132,7 @@ __device__ __forceinline__ void store32(void* out, size_t row, int n0, int cols,
 }
 
 template <typename T, int MODE, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
              const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1, Params p) {
     constexpr bool A_MN = MODE == DW, B_MN = MODE != FWD;
@@ -174,6 +175,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
     tc_fence_after();
     const uint32_t tmem_base = bars->tmem_base;
     volatile int* abort_flag = &bars->abort;
+    wait_previous_grid();
 
     if (warp == 0 && lane == 0) {
         // ------------------------------------------------------------ producer (both CTAs)
@@ -340,6 +342,7 @@ __global__ void __launch_bounds__(256)
 gate_backward_kernel(const uint4* __restrict__ dH, const uint4* __restrict__ G, const uint4* __restrict__ U,
                      uint4* __restrict__ dG, uint4* __restrict__ dU, uint64_t n8) {
     const uint64_t step = (uint64_t)gridDim.x * blockDim.x;
+    wait_previous_grid();
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += step) {
         const uint4 vh = __ldg(dH + i), vg = __ldg(G + i), vu = __ldg(U + i);
         const uint32_t h[4] = {vh.x, vh.y, vh.z, vh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
@@ -382,14 +385,19 @@ static int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMa
         lc.gridDim = dim3(info->sm_count & ~1);
         lc.blockDim = dim3(THREADS);
         lc.dynamicSmemBytes = SMEM_BYTES;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim = {2, 1, 1};
+        lc.attrs = at;
+        lc.numAttrs = 1;
         QG_CUDA(cudaOccupancyMaxActiveClusters(&res, gated_kernel<T, MODE, ACT>, &lc));
         if (res < 1) res = 1;
         resident[dev & 63] = res;
     }
     const int tiles = p.tiles_m * p.tiles_n;
     const int pairs = tiles < res ? tiles : res;
-    gated_kernel<T, MODE, ACT><<<2 * pairs, THREADS, SMEM_BYTES, stream>>>(a0, a1, b0, b1, p);
-    QG_CUDA(cudaGetLastError());
+    QG_CUDA(launch_overlapped(gated_kernel<T, MODE, ACT>, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, 2, a0, a1, b0,
+                              b1, p));
     return QG_OK;
 }
 
@@ -448,9 +456,9 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     auto* vu = static_cast<const uint4*>(U);
     auto* og = static_cast<uint4*>(dG);
     auto* ou = static_cast<uint4*>(dU);
-    if (act == QG_ACT_SILU) gate_backward_kernel<T, QG_ACT_SILU><<<grid, 256, 0, stream>>>(vh, vg, vu, og, ou, n8);
-    else gate_backward_kernel<T, QG_ACT_GELU_TANH><<<grid, 256, 0, stream>>>(vh, vg, vu, og, ou, n8);
-    QG_CUDA(cudaGetLastError());
+    QG_CUDA(launch_overlapped(act == QG_ACT_SILU ? gate_backward_kernel<T, QG_ACT_SILU>
+                                                 : gate_backward_kernel<T, QG_ACT_GELU_TANH>,
+                              dim3(grid), dim3(256), 0, stream, 1, vh, vg, vu, og, ou, n8));
     CUtensorMap a0, a1, b0, b1;
     if (dX) {
         if ((rc = make_map(&a0, dG, M, N, BM)) || (rc = make_map(&a1, dU, M, N, BM)) ||

@@ -63,6 +63,16 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
     return w;
 }
 
+// Two values to two codes, the first in the low nibble.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t w;
+    asm("{\n\t.reg .b8 a;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "mov.b32 %0, {a, a, a, a};\n\t}"
+        : "=r"(w) : "f"(lo), "f"(hi));
+    return w & 0xFFu;
+}
+
 // The magnitude of e2m1 code c (its low three bits) as fp32 bits: 0, 0.5, then
 // exponent field (c >> 1) + 126 with the low code bit as the top mantissa bit.
 __device__ __forceinline__ float code_value(uint32_t c) {

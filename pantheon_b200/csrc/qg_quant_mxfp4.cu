@@ -9,6 +9,7 @@
 // first use.
 #include "qg_common.cuh"
 #include "qg_formats.cuh"
+#include "qg_launch.cuh"
 #include "qg_mxfp4.cuh"
 
 #include <cuda_bf16.h>
@@ -53,6 +54,7 @@ quant_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q, uint
     const int row_groups = (M + 127) / 128 * (128 / ROWS);   // the rows that pad the last atom get zero scales
     const uint64_t units = (uint64_t)segs * (uint64_t)row_groups;
     const uint64_t step = (uint64_t)gridDim.x * (THREADS / 32);
+    wait_previous_grid();
     for (uint64_t u = (uint64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); u < units; u += step) {
         const int rg = (int)(u / (uint32_t)segs);
         const int k0 = (int)(u - (uint64_t)rg * (uint32_t)segs) * SEG + lane * 8;
@@ -92,6 +94,7 @@ dequant_kernel(const uint8_t* __restrict__ Q, const uint8_t* __restrict__ SF, T*
     const int kchunks = (K + ATOM_K - 1) / ATOM_K;
     const uint64_t total = (uint64_t)M * (uint32_t)words;
     const uint64_t step = (uint64_t)gridDim.x * THREADS;
+    wait_previous_grid();
     for (uint64_t i = (uint64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += step) {
         const int r = (int)(i / (uint32_t)words);
         const int c = (int)(i - (uint64_t)r * (uint32_t)words);
@@ -133,9 +136,8 @@ static int launch_quant(const void* X, int64_t ldx, void* Q, void* SF, int M, in
     const T* x = static_cast<const T*>(X);
     uint8_t* q = static_cast<uint8_t*>(Q);
     uint8_t* sf = static_cast<uint8_t*>(SF);
-    if (vec) quant_kernel<T, true><<<grid, THREADS, 0, s>>>(x, ldx, q, sf, M, K);
-    else quant_kernel<T, false><<<grid, THREADS, 0, s>>>(x, ldx, q, sf, M, K);
-    QG_CUDA(cudaGetLastError());
+    QG_CUDA(launch_overlapped(vec ? quant_kernel<T, true> : quant_kernel<T, false>, dim3(grid), dim3(THREADS), 0, s, 1, x,
+                              ldx, q, sf, M, K));
     return QG_OK;
 }
 
@@ -177,10 +179,11 @@ int dequant_mxfp4(const void* Q, const void* SF, void* Y, int out_type, int M, i
     const uint8_t* q = static_cast<const uint8_t*>(Q);
     const uint8_t* sf = static_cast<const uint8_t*>(SF);
     if (out_type == QG_OUT_F32)
-        mx::dequant_kernel<float><<<grid, mx::THREADS, 0, s>>>(q, sf, static_cast<float*>(Y), M, K);
+        QG_CUDA(launch_overlapped(mx::dequant_kernel<float>, dim3(grid), dim3(mx::THREADS), 0, s, 1, q, sf,
+                                  static_cast<float*>(Y), M, K));
     else
-        mx::dequant_kernel<__nv_bfloat16><<<grid, mx::THREADS, 0, s>>>(q, sf, static_cast<__nv_bfloat16*>(Y), M, K);
-    QG_CUDA(cudaGetLastError());
+        QG_CUDA(launch_overlapped(mx::dequant_kernel<__nv_bfloat16>, dim3(grid), dim3(mx::THREADS), 0, s, 1, q, sf,
+                                  static_cast<__nv_bfloat16*>(Y), M, K));
     return QG_OK;
 }
 
