@@ -222,7 +222,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, uint64_t* tmem_ful
         tmem_ld_wait_regs(r1);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tmem_empty);
+        if (lane == 0) mbar_arrive_relaxed(tmem_empty);     // orders TMEM reads only
 
         const int m = mt * tile_rows + row0 + row;
         if constexpr (!GATED) {
@@ -416,7 +416,10 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 // halve: each CTA's TMEM holds those of its own rows of A and of all 256 rows of
 // B.  Protocol beyond the single CTA's:
 //   * codes of both CTAs complete on the even CTA's `full` barrier;
-//   * scales go by blocks of 512 K with rings of their own, in shared memory
+//   * a stage is 512 K (two boxes per operand): the MMA thread's waits cost it
+//     about 350 clocks a stage, against 1024 clocks of MMAs here and 512 with
+//     256 K per stage (111 us at 4096x8192x8192);
+//   * scales have rings of their own, in shared memory
 //     (filled ahead of the codes by warp 22, freed by the writers) and in TMEM
 //     (freed by a commit of the MMAs that read it), so neither a load nor the
 //     writers' round trip lies between a freed code stage and its MMAs;
@@ -426,11 +429,12 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 //     every access of its thread, took 1400 clocks per K block (157 us in all at
 //     4096x8192x8192);
 //   * the MMA thread commits `empty` and `tmem_full` to both CTAs (plain commits).
-constexpr int P_STAGES = 6;                                    // code ring
-constexpr int P_OP_BYTES = 128 * BK_BYTES;                     // 16 KB: either operand of a CTA
-constexpr int P_SFK = 2;                                       // K blocks per scale block
+constexpr int P_KB = 2;                                        // 256-element K blocks per stage
+constexpr int P_STAGES = 3;                                    // code ring
+constexpr int P_BLOCK_BYTES = 128 * BK_BYTES;                  // 16 KB: a K block of either operand of a CTA
+constexpr int P_OP_BYTES = P_KB * P_BLOCK_BYTES;
 constexpr int P_SF_STAGES = 4;                                 // scale ring in shared memory
-constexpr int P_SFA_BYTES = P_SFK * SFA_BYTES, P_SFB_BYTES = P_SFK * SFB_BYTES;
+constexpr int P_SFA_BYTES = P_KB * SFA_BYTES, P_SFB_BYTES = P_KB * SFB_BYTES;
 constexpr int P_SF_BYTES = P_SFA_BYTES + P_SFB_BYTES;          // 6 KB
 constexpr int P_SF_COLS = P_SF_BYTES / 128;                    // 48 TMEM columns: A's four atoms, then B's per 128 K
 constexpr int P_SF_SLOTS = (TMEM_COLS - BN) / P_SF_COLS;       // 5: the scale ring in TMEM
@@ -463,10 +467,6 @@ __device__ __forceinline__ void umma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc,
         : "memory");
 }
 
-__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
 // One commit that arrives on the same barrier of both CTAs of the pair.
 __device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
@@ -496,7 +496,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     const int tiles_n = (p.N + TN - 1) / TN;
     const int tiles = tiles_m * tiles_n;
     const int nk = (p.K + BK - 1) / BK;
-    const int ns = (nk + P_SFK - 1) / P_SFK;
+    const int ns = (nk + P_KB - 1) / P_KB;
     const int kchunks = (p.K + ATOM_K - 1) / ATOM_K;
     const int a_row_blocks = (p.M + 127) / 128, b_row_blocks = (p.N + 127) / 128;
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -544,12 +544,18 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
             tile_coords(t, tiles_m, tiles_n, p.group_m, mt, nt);
             const CUtensorMap* b = GATED && !leader ? &tmB2 : &tmB;
             const int b_row = GATED ? nt * 128 : nt * BN + (int)rank * 128;
-            for (int kb = 0; kb < nk; ++kb) {
+            for (int kb = 0; kb < nk; kb += P_KB) {
                 if (!mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER)) { ok = false; break; }
-                if (leader) mbar_arrive_expect_tx(&bars->full[stage], 4 * P_OP_BYTES);
+                const int n = min(P_KB, nk - kb);
+                if (leader) mbar_arrive_expect_tx(&bars->full[stage], (uint32_t)n * 4 * P_BLOCK_BYTES);
                 const uint32_t full = mapa_shared(smem_u32(&bars->full[stage]), 0);
-                tma_load_2d_pair(sA + stage * P_OP_BYTES, &tmA, full, kb * BK_BYTES, mt * 2 * BM + (int)rank * BM);
-                tma_load_2d_pair(sB + stage * P_OP_BYTES, b, full, kb * BK_BYTES, b_row);
+#pragma unroll
+                for (int j = 0; j < P_KB; ++j)
+                    if (j < n) {
+                        tma_load_2d_pair(sA + stage * P_OP_BYTES + j * P_BLOCK_BYTES, &tmA, full, (kb + j) * BK_BYTES,
+                                         mt * 2 * BM + (int)rank * BM);
+                        tma_load_2d_pair(sB + stage * P_OP_BYTES + j * P_BLOCK_BYTES, b, full, (kb + j) * BK_BYTES, b_row);
+                    }
                 armed |= 1u << stage;
                 armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
                 if (++stage == P_STAGES) { stage = 0; phase ^= 1u; }
@@ -576,8 +582,8 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                                         : p.sfb + (size_t)(nt * 2 + 1 < b_row_blocks ? nt * 2 + 1 : 0) * kchunks * ATOM_BYTES;
             for (int sb = 0; sb < ns; ++sb) {
                 if (!mbar_wait(&bars->sf_empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER)) { ok = false; break; }
-                const uint32_t atoms = (uint32_t)min(P_SFK * ATOMS, kchunks - sb * P_SFK * ATOMS) * ATOM_BYTES;
-                const size_t at = (size_t)sb * P_SFK * ATOMS * ATOM_BYTES;
+                const uint32_t atoms = (uint32_t)min(P_KB * ATOMS, kchunks - sb * P_KB * ATOMS) * ATOM_BYTES;
+                const size_t at = (size_t)sb * P_KB * ATOMS * ATOM_BYTES;
                 uint64_t* full = &bars->sf_full[stage];
                 mbar_arrive_expect_tx(full, 3 * atoms);
                 bulk_load(sSFA + stage * P_SFA_BYTES, sfa + at, atoms, full);
@@ -602,30 +608,32 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         int iter = 0;
         for (int t = pair; t < tiles && ok; t += pairs, ++iter) {
             if (!warp_wait(&bars->tmem_empty, (iter & 1) ^ 1u, abort_flag, p.status, SITE_MMA_TMEM)) { ok = false; break; }
-            for (int kb = 0; kb < nk; ++kb) {
-                const int sub = kb % P_SFK;
-                if (sub == 0 && !warp_wait(&bars->sc_ready[slot], slot_phase, abort_flag, p.status, SITE_MMA_SF)) { ok = false; break; }
-                if (!warp_wait(&bars->full[stage], phase, abort_flag, p.status, SITE_MMA_FULL)) { ok = false; break; }
+            for (int sb = 0; sb < ns; ++sb) {
+                if (!warp_wait(&bars->sc_ready[slot], slot_phase, abort_flag, p.status, SITE_MMA_SF) ||
+                    !warp_wait(&bars->full[stage], phase, abort_flag, p.status, SITE_MMA_FULL)) {
+                    ok = false;
+                    break;
+                }
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t sfa_col = tmem_base + BN + slot * P_SF_COLS + sub * 8;
-                    const uint32_t sfb_col = tmem_base + BN + slot * P_SF_COLS + P_SFK * 8 + sub * 16;
+                    const uint32_t sfa_col = tmem_base + BN + slot * P_SF_COLS, sfb_col = sfa_col + P_KB * 8;
                     const uint64_t ad = a_desc0 + stage * (P_OP_BYTES >> 4), bd = b_desc0 + stage * (P_OP_BYTES >> 4);
-                    const int steps = (p.K - kb * BK + UMMA_K - 1) / UMMA_K;       // 4 but for the last block
+                    const int steps = (p.K - sb * P_KB * BK + UMMA_K - 1) / UMMA_K;      // all 8 but for the last stage
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k)
-                        if (k < steps)
-                            umma_mxf4_pair(tmem_base, ad + k * (UMMA_K / 2 >> 4), bd + k * (UMMA_K / 2 >> 4),
-                                           (k & 1) ? IDESC2 : IDESC0, sfa_col + 4 * (k >> 1), sfb_col + 8 * (k >> 1),
-                                           (kb | k) != 0 ? 1u : 0u);
+                    for (int k = 0; k < P_KB * BK / UMMA_K; ++k)
+                        if (k < steps) {
+                            const uint64_t at = (uint64_t)((k / 4) * (P_BLOCK_BYTES >> 4) + (k % 4) * (UMMA_K / 2 >> 4));
+                            umma_mxf4_pair(tmem_base, ad + at, bd + at, (k & 1) ? IDESC2 : IDESC0, sfa_col + 4 * (k >> 1),
+                                           sfb_col + 8 * (k >> 1), (sb | k) != 0 ? 1u : 0u);
+                        }
                     umma_commit_both(&bars->empty[stage]);
-                    if (sub + 1 == P_SFK || kb + 1 == nk) umma_commit_both(&bars->sc_empty[slot]);
-                    if (kb + 1 == nk) umma_commit_both(&bars->tmem_full);
+                    umma_commit_both(&bars->sc_empty[slot]);
+                    if (sb + 1 == ns) umma_commit_both(&bars->tmem_full);
                 }
                 __syncwarp();
                 issued = true;
                 if (++stage == P_STAGES) { stage = 0; phase ^= 1u; }
-                if ((sub + 1 == P_SFK || kb + 1 == nk) && ++slot == P_SF_SLOTS) { slot = 0; slot_phase ^= 1u; }
+                if (++slot == P_SF_SLOTS) { slot = 0; slot_phase ^= 1u; }
             }
         }
         if (!ok && issued && elect_one()) {
@@ -649,8 +657,8 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
             const uint4* sfb = reinterpret_cast<const uint4*>(sSFB + stage * P_SFB_BYTES) + lane;
             uint32_t va[16], vb[16], vc[16];
 #pragma unroll
-            for (int k = 0; k < P_SFK * ATOMS; ++k) {
-                const uint4 x = sfa[k * 32], y = sfb[k * 32], z = sfb[(P_SFK * ATOMS + k) * 32];
+            for (int k = 0; k < P_KB * ATOMS; ++k) {
+                const uint4 x = sfa[k * 32], y = sfb[k * 32], z = sfb[(P_KB * ATOMS + k) * 32];
                 uint32_t* d = k < 2 ? vb + 8 * k : vc + 8 * (k - 2);
                 va[4 * k] = x.x; va[4 * k + 1] = x.y; va[4 * k + 2] = x.z; va[4 * k + 3] = x.w;
                 d[0] = y.x; d[1] = y.y; d[2] = y.z; d[3] = y.w;

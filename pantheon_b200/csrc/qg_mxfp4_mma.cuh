@@ -22,6 +22,13 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t M, uint32_t N, uint32
     return make_idesc_bs(/*e2m1*/ 1, /*e2m1*/ 1, /*ue8m0*/ 1, M, N) | (sf_id << 4) | (sf_id << 29);
 }
 
+// Arrive on an mbarrier of the cluster without release: for handing over TMEM
+// contents, complete after tcgen05.wait and ordered by the tcgen05 fences on
+// both sides.  Not for shared or global memory.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
