@@ -775,10 +775,13 @@ static int check_mx(const char* name, const void* A, const void* SFA, const void
 
 } // namespace mx
 
-// Which kernel: the one for few rows up to 32 rows, and while 128 x 256 tiles
-// would leave half of the SMs idle.
-static bool use_rows(int M, int cols) {
-    return M <= 32 || 2 * (int64_t)ceil_div(M, mx::BM) * ceil_div(cols, mx::BN) <= 148;
+// Which kernel: the one for few rows up to 64 rows (32 of a gated product, whose
+// tiles are half as wide), and while 128 x 256 tiles would leave half of the SMs
+// idle; then single CTAs up to 128 rows, pairs above.  Measured at K=8192, few
+// rows / single / pairs: 64x28672 24.6 / 25.6 / 30.3 us, 128x28672 28.2 / 27.8 /
+// 33.2; gated at K=4096: 64x14336 16.5 / 15.5 / 19.5, 128x14336 19.0 / 16.7 / 20.4.
+static bool use_rows(int M, int cols, bool is_gated) {
+    return M <= (is_gated ? 32 : 64) || 2 * (int64_t)ceil_div(M, mx::BM) * ceil_div(cols, mx::BN) <= 148;
 }
 
 int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, void* C, int out_type, int M, int N,
@@ -787,7 +790,7 @@ int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, v
     if (rc) return rc;
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFB), nullptr, C, nullptr,
                      nullptr, 1, false};
-    const bool few = use_rows(M, N);
+    const bool few = use_rows(M, N, false);
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)C % 2 == 0, "qg_gemm_mxfp4: C is not aligned to its element");
@@ -812,7 +815,7 @@ int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void*
     QG_CHECK_ARG(act == QG_ACT_SILU || act == QG_ACT_GELU_TANH, "qg_gemm_gated_mxfp4: unknown activation %d", act);
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFG),
                      static_cast<const uint8_t*>(SFU), H, static_cast<uint8_t*>(SFH), nullptr, 1, false};
-    const bool silu = act == QG_ACT_SILU, few = use_rows(M, 2 * N);
+    const bool silu = act == QG_ACT_SILU, few = use_rows(M, 2 * N, true);
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)H % 2 == 0, "qg_gemm_gated_mxfp4: H is not aligned to its element");

@@ -7,7 +7,6 @@ to the sm_100a kernels in libpantheon_qgemm.so; there is no other path.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
@@ -187,16 +186,27 @@ def gen_nvfp4(M: int, N: int, K: int, seed: int, tid0: int = 0, device="cuda"):
     return A, sfa, B, sfb, g
 
 
-def _on_device(t: torch.Tensor):
-    """A context in which t's device is the current one (a launch goes to the current device)."""
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+def _launch(entry: str, like: torch.Tensor, *args):
+    """A C entry on like's device and that device's current stream; tensors go as their addresses."""
+    fn = getattr(load_library(), entry)
+    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    index = like.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(index)   # current_stream(index).cuda_stream, without its object
+    if index == torch.cuda.current_device():
+        code = fn(*args, stream)
+    else:   # a launch goes to the current device
+        with torch.cuda.device(index):
+            code = fn(*args, stream)
+    if code:
+        check(entry, code)
 
 
 def _require(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, like: torch.Tensor):
     """A contiguous CUDA tensor of this type and shape on like's device."""
+    if t.dtype is dtype and t.shape == shape and t.is_cuda and t.get_device() == like.get_device() and t.is_contiguous():
+        return
     _require_cuda(t)
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != like.device:
-        raise ValueError(f"{name} must be {dtype} {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    raise ValueError(f"{name} must be {dtype} {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 _MX_IN_TYPES = {torch.bfloat16: QG_OUT_BF16, torch.float16: QG_OUT_F16, torch.float32: QG_OUT_F32}
@@ -227,9 +237,7 @@ def quant_mxfp4(X: torch.Tensor):
         raise ValueError(f"quant_mxfp4: rows must not overlap (row stride {X.stride(0)} < K={K})")
     sf = torch.empty((mxfp4_sf_bytes(M, K),), dtype=torch.uint8, device=X.device)
     q = torch.empty((M, (K + 31) // 32 * 16), dtype=torch.uint8, device=X.device)
-    with _on_device(X):
-        check("qg_quant_mxfp4", load_library().qg_quant_mxfp4(_ptr(X), _MX_IN_TYPES[X.dtype], X.stride(0) if M > 1 else K,
-                                                               _ptr(q), _ptr(sf), M, K, _stream(X.device)))
+    _launch("qg_quant_mxfp4", X, X, _MX_IN_TYPES[X.dtype], X.stride(0) if M > 1 else K, q, sf, M, K)
     return q, sf
 
 
@@ -237,10 +245,10 @@ def _mx_operand(name: str, Q: torch.Tensor, SF: torch.Tensor, like: torch.Tensor
     """(rows, K) of an MXFP4 operand."""
     if Q.dim() != 2:
         raise ValueError(f"{name}: codes must be 2-D, got {list(Q.shape)}")
-    rows, K = Q.shape[0], 2 * Q.shape[1]
-    _require(name, Q, torch.uint8, (rows, K // 2), like)
-    _require(f"{name}'s scales", SF, torch.uint8, (mxfp4_sf_bytes(rows, K),), like)
-    return rows, K
+    rows, half = Q.shape
+    _require(name, Q, torch.uint8, (rows, half), like)
+    _require(name, SF, torch.uint8, (mxfp4_sf_bytes(rows, 2 * half),), like)
+    return rows, 2 * half
 
 
 def dequant_mxfp4(Q: torch.Tensor, SF: torch.Tensor, out_type: int = QG_OUT_BF16) -> torch.Tensor:
@@ -249,9 +257,7 @@ def dequant_mxfp4(Q: torch.Tensor, SF: torch.Tensor, out_type: int = QG_OUT_BF16
     if out_type not in (QG_OUT_BF16, QG_OUT_F32):
         raise ValueError(f"dequant_mxfp4: out_type {out_type} (bf16 or f32)")
     out = torch.empty((M, K), dtype=_OUT_DTYPES[out_type], device=Q.device)
-    with _on_device(Q):
-        check("qg_dequant_mxfp4", load_library().qg_dequant_mxfp4(_ptr(Q), _ptr(SF), _ptr(out), out_type, M, K,
-                                                                   _stream(Q.device)))
+    _launch("qg_dequant_mxfp4", Q, Q, SF, out, out_type, M, K)
     return out
 
 
@@ -271,9 +277,7 @@ def gemm_mxfp4(A: torch.Tensor, sfa: torch.Tensor, B: torch.Tensor, sfb: torch.T
         out = torch.empty((M, N), dtype=_OUT_DTYPES[out_type], device=A.device)
     else:
         _require("gemm_mxfp4: out", out, _OUT_DTYPES[out_type], (M, N), A)
-    with _on_device(A):
-        check("qg_gemm_mxfp4", load_library().qg_gemm_mxfp4(_ptr(A), _ptr(sfa), _ptr(B), _ptr(sfb), _ptr(out), out_type,
-                                                             M, N, K, _stream(A.device)))
+    _launch("qg_gemm_mxfp4", A, A, sfa, B, sfb, out, out_type, M, N, K)
     return out
 
 
@@ -298,10 +302,7 @@ def gemm_gated_mxfp4(A: torch.Tensor, sfa: torch.Tensor, Wg: torch.Tensor, sfg: 
         out = torch.empty((M, N), dtype=_OUT_DTYPES[out_type], device=A.device)
     else:
         raise ValueError(f"gemm_gated_mxfp4: out_type {out_type} (bf16, f32 or mxfp4)")
-    with _on_device(A):
-        check("qg_gemm_gated_mxfp4",
-              load_library().qg_gemm_gated_mxfp4(_ptr(A), _ptr(sfa), _ptr(Wg), _ptr(sfg), _ptr(Wu), _ptr(sfu), _ptr(out),
-                                                 _ptr(sfh), out_type, act, M, N, K, _stream(A.device)))
+    _launch("qg_gemm_gated_mxfp4", A, A, sfa, Wg, sfg, Wu, sfu, out, sfh, out_type, act, M, N, K)
     return (out, sfh) if out_type == QG_OUT_MXFP4 else out
 
 
@@ -319,10 +320,7 @@ def _gated_shape(entry: str, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor
 def _gemm_gated(entry: str, dtype: torch.dtype, X, Wg, Wu, act, keep):
     M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
     out = [torch.empty((M, N), dtype=dtype, device=X.device) for _ in range(3 if keep else 1)]
-    with _on_device(X):
-        check(entry, getattr(load_library(), entry)(_ptr(X), _ptr(Wg), _ptr(Wu), _ptr(out[0]),
-                                                    _ptr(out[1]) if keep else None, _ptr(out[2]) if keep else None,
-                                                    act, M, N, K, _stream(X.device)))
+    _launch(entry, X, X, Wg, Wu, out[0], out[1] if keep else None, out[2] if keep else None, act, M, N, K)
     return tuple(out) if keep else out[0]
 
 
@@ -337,10 +335,7 @@ def _gemm_gated_backward(entry: str, dtype: torch.dtype, dH, X, Wg, Wu, G, U, ac
         workspace = torch.empty((4 * M * N,), dtype=torch.uint8, device=X.device)
     else:
         _require(f"{entry}: workspace", workspace, torch.uint8, tuple(workspace.shape), X)
-    with _on_device(X):
-        check(entry, getattr(load_library(), entry)(_ptr(dH), _ptr(X), _ptr(Wg), _ptr(Wu), _ptr(G), _ptr(U), _ptr(dX),
-                                                    _ptr(dWg), _ptr(dWu), act, M, N, K, _ptr(workspace),
-                                                    workspace.numel(), _stream(X.device)))
+    _launch(entry, X, dH, X, Wg, Wu, G, U, dX, dWg, dWu, act, M, N, K, workspace, workspace.numel())
     return dX, dWg, dWu
 
 
