@@ -73,13 +73,5 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return w & 0xFFu;
 }
 
-// The magnitude of e2m1 code c (its low three bits) as fp32 bits: 0, 0.5, then
-// exponent field (c >> 1) + 126 with the low code bit as the top mantissa bit.
-__device__ __forceinline__ float code_value(uint32_t c) {
-    const uint32_t m = c & 7u;
-    const uint32_t mag = m < 2 ? (m ? 0x3F000000u : 0u) : ((m >> 1) + 126u) << 23 | (m & 1u) << 22;
-    return __uint_as_float(mag | (c & 8u) << 28);
-}
-
 } // namespace mx
 } // namespace qg

@@ -1,12 +1,13 @@
 // qg_quant_mxfp4.cu -- a tensor into MXFP4 (qg_mxfp4.cuh) and back.
 //
 // Both directions are streams: quantisation reads M K values and writes
-// M K (1/2 + 1/32) bytes, so the memory system bounds them.  A warp takes 256
-// consecutive columns of ROWS rows: a lane holds eight of them (one 16-byte
-// load of a 2-byte type), the maximum of a block is two shuffles over its four
-// lanes, the lane's eight codes are one 4-byte store and a row's four scales of
-// an atom are one 4-byte store.  The ROWS loads of a lane are issued before the
-// first use.
+// M K (1/2 + 1/32) bytes, so the memory system bounds them, if the arithmetic
+// stays near six instructions per value.  A lane holds 32 bytes of a row (sixteen
+// 2-byte values or eight fp32), a warp 1 KB of each of ROWS rows; all loads of a
+// lane are issued before the first use.  Magnitudes are compared as integers of
+// their own type (two per instruction for 2-byte types), a block's maximum is one
+// or two shuffles, scaling by a power of two is exact, and the conversion to codes
+// is the hardware's.
 #include "qg_common.cuh"
 #include "qg_formats.cuh"
 #include "qg_launch.cuh"
@@ -14,99 +15,183 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace qg {
 namespace mx {
 
-constexpr int SEG = 256;        // columns of a warp
+constexpr int SEG = 256;        // columns of a warp (dequantisation)
 constexpr int ROWS = 4;         // rows of a warp
 constexpr int THREADS = 256;
 
-template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+// A lane's 32 bytes of a row.
+template <typename T>
+struct Raw {
+    static constexpr int N = 32 / sizeof(T);        // values
+    uint32_t w[8];
+};
 
-// The lane's eight values; `n` of them exist, the others are zero.
+// `n` of the values exist, the others are zero.  VEC: rows start on 16 bytes.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* src, int n, float (&v)[8]) {
-    if (VEC && n == 8) {
-        constexpr int W = 8 * sizeof(T) / 16;
-        uint4 raw[W];
+__device__ __forceinline__ void load(const T* src, int n, Raw<T>& v) {
+    constexpr int N = Raw<T>::N;
+    if (VEC && n == N) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-        const T* t = reinterpret_cast<const T*>(raw);
+        for (int i = 0; i < 2; ++i) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(src) + i);
+            v.w[4 * i] = q.x; v.w[4 * i + 1] = q.y; v.w[4 * i + 2] = q.z; v.w[4 * i + 3] = q.w;
+        }
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
+        for (int i = 0; i < 8; ++i) v.w[i] = i < n ? __ldg(reinterpret_cast<const uint32_t*>(src) + i) : 0u;
     } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+        if (n == N && (reinterpret_cast<uintptr_t>(src) & 2) == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(src[i]) : 0.0f;
+            for (int i = 0; i < 8; ++i) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+        } else if (n == N) {
+            // off by half a word: the words between, joined with their neighbours
+            uint32_t lo = __ldg(h);
+#pragma unroll
+            for (int i = 0; i < 7; ++i) {
+                const uint32_t next = __ldg(reinterpret_cast<const uint32_t*>(h + 1) + i);
+                v.w[i] = lo | next << 16;
+                lo = next >> 16;
+            }
+            v.w[7] = lo | (uint32_t)__ldg(h + 15) << 16;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v.w[i] = (2 * i < n ? (uint32_t)__ldg(h + 2 * i) : 0u) |
+                         (2 * i + 1 < n ? (uint32_t)__ldg(h + 2 * i + 1) << 16 : 0u);
+        }
     }
+}
+
+// Bits of the largest magnitude as its own type's integer: magnitudes of one type
+// order as integers, NaN above infinity above the rest.
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(const Raw<T>& v) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        if constexpr (sizeof(T) == 4) m = __vimax3_u32(m, v.w[i] & 0x7FFFFFFFu, v.w[i + 1] & 0x7FFFFFFFu);
+        else m = __vimax3_u16x2(m, v.w[i] & 0x7FFF7FFFu, v.w[i + 1] & 0x7FFF7FFFu);
+    }
+    return sizeof(T) == 4 ? m : max(m & 0xFFFFu, m >> 16);
+}
+template <typename T> __device__ __forceinline__ uint32_t f32_bits(uint32_t m);
+template <> __device__ __forceinline__ uint32_t f32_bits<float>(uint32_t m) { return m; }
+template <> __device__ __forceinline__ uint32_t f32_bits<__nv_bfloat16>(uint32_t m) { return m << 16; }
+template <> __device__ __forceinline__ uint32_t f32_bits<__half>(uint32_t m) {
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+}
+
+// Value i of the lane.
+template <typename T>
+__device__ __forceinline__ float value(const Raw<T>& v, int i) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(v.w[i]);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        return __uint_as_float((i & 1) ? v.w[i / 2] & 0xFFFF0000u : v.w[i / 2] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)((i & 1) ? v.w[i / 2] >> 16 : v.w[i / 2] & 0xFFFFu)));
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 quant_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q, uint8_t* __restrict__ SF, int M, int K) {
+    constexpr int N = Raw<T>::N;                              // 16 or 8 values, 2 or 4 lanes per block
     const int lane = threadIdx.x & 31;
     const int kp = (K + BLOCK - 1) / BLOCK * BLOCK;          // columns that have codes
     const int kchunks = (K + ATOM_K - 1) / ATOM_K;
-    const int segs = (kchunks * ATOM_K + SEG - 1) / SEG;
+    const int segs = (kchunks * ATOM_K + 32 * N - 1) / (32 * N);
     const int row_groups = (M + 127) / 128 * (128 / ROWS);   // the rows that pad the last atom get zero scales
     const uint64_t units = (uint64_t)segs * (uint64_t)row_groups;
-    const uint64_t step = (uint64_t)gridDim.x * (THREADS / 32);
     wait_previous_grid();
-    for (uint64_t u = (uint64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); u < units; u += step) {
-        const int rg = (int)(u / (uint32_t)segs);
-        const int k0 = (int)(u - (uint64_t)rg * (uint32_t)segs) * SEG + lane * 8;
-        const int r0 = rg * ROWS;
-        const int n = min(8, max(0, K - k0));
-        float v[ROWS][8];
+    const uint64_t u = (uint64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+    if (u >= units) return;
+    const int rg = (int)(u / (uint32_t)segs);
+    const int k0 = (int)(u - (uint64_t)rg * (uint32_t)segs) * (32 * N) + lane * N;
+    const int r0 = rg * ROWS;
+    const int n = min(N, max(0, K - k0));
+    Raw<T> v[ROWS];
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i)
-            load8<T, VEC>(X + (int64_t)(r0 + i) * ldx + k0, r0 + i < M ? n : 0, v[i]);
+    for (int i = 0; i < ROWS; ++i) load<T, VEC>(X + (int64_t)(r0 + i) * ldx + k0, r0 + i < M ? n : 0, v[i]);
+    uint8_t* q = Q + (size_t)r0 * (kp / 2) + k0 / 2;
+    // the ROWS rows of a unit follow one another in their atom, 16 bytes apart
+    uint8_t* sf = SF + sf_offset(r0, k0 / BLOCK, kchunks);
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            uint32_t amax = 0;
+    for (int i = 0; i < ROWS; ++i) {
+        uint32_t m = max_bits(v[i]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const uint32_t s = scale_byte(amax);
-            const float inv = inv_scale(s == 255 ? 0 : s);
+        for (int o = 1; o < BLOCK / N; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const uint32_t s = scale_byte(f32_bits<T>(m));
+        const float inv = inv_scale(s == 255 ? 0 : s);
+        uint32_t w[N / 8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= inv;
-            const uint32_t w = s == 255 ? 0u : pack8(v[i]);
-            if (r0 + i < M && k0 < kp)
-                *reinterpret_cast<uint32_t*>(Q + (size_t)(r0 + i) * (kp / 2) + k0 / 2) = w;
-            // lanes 0, 4, 8, 12 (16, 20, 24, 28) hold the four scales of one atom row
-            const uint32_t pair = s | __shfl_down_sync(0xffffffffu, s, 4) << 8;
-            const uint32_t four = pair | __shfl_down_sync(0xffffffffu, pair, 8) << 16;
-            if ((lane & 15) == 0 && k0 / ATOM_K < kchunks)
-                *reinterpret_cast<uint32_t*>(SF + sf_offset(r0 + i, k0 / BLOCK, kchunks)) = four;
+        for (int g = 0; g < N / 8; ++g) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = value(v[i], 8 * g + j) * inv;
+            w[g] = s == 255 ? 0u : pack8(f);
         }
+        if (r0 + i < M && k0 < kp) {
+            if constexpr (N == 16) *reinterpret_cast<uint2*>(q + (size_t)i * (kp / 2)) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t*>(q + (size_t)i * (kp / 2)) = w[0];
+        }
+        // a row's four scales of an atom lie BLOCK / N lanes apart
+        const uint32_t pair = s | __shfl_down_sync(0xffffffffu, s, BLOCK / N) << 8;
+        const uint32_t four = pair | __shfl_down_sync(0xffffffffu, pair, 2 * BLOCK / N) << 16;
+        if ((lane & (ATOM_K / N - 1)) == 0 && k0 < kchunks * ATOM_K) *reinterpret_cast<uint32_t*>(sf + 16 * i) = four;
     }
 }
 
+// Two codes to two fp32 values, exactly (through fp16).
+__device__ __forceinline__ float2 unpack2(uint32_t byte) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
+        : "=r"(h) : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// The reverse, in the same shape: a lane's four bytes of a row are eight values.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 dequant_kernel(const uint8_t* __restrict__ Q, const uint8_t* __restrict__ SF, T* __restrict__ Y, int M, int K) {
-    const int words = K / 8;                                   // 4-byte code words of a row
+    const int lane = threadIdx.x & 31;
     const int kchunks = (K + ATOM_K - 1) / ATOM_K;
-    const uint64_t total = (uint64_t)M * (uint32_t)words;
-    const uint64_t step = (uint64_t)gridDim.x * THREADS;
+    const int segs = (K + SEG - 1) / SEG;
+    const uint64_t units = (uint64_t)segs * (uint64_t)((M + ROWS - 1) / ROWS);
     wait_previous_grid();
-    for (uint64_t i = (uint64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += step) {
-        const int r = (int)(i / (uint32_t)words);
-        const int c = (int)(i - (uint64_t)r * (uint32_t)words);
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(Q) + i);
-        const float s = scale_value(__ldg(SF + sf_offset(r, c >> 2, kchunks)));
+    const uint64_t u = (uint64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+    if (u >= units) return;
+    const int rg = (int)(u / (uint32_t)segs);
+    const int k0 = (int)(u - (uint64_t)rg * (uint32_t)segs) * SEG + lane * 8;
+    const int r0 = rg * ROWS;
+    if (k0 >= K) return;
+    uint32_t w[ROWS], s[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + i < M ? r0 + i : M - 1;
+        w[i] = __ldg(reinterpret_cast<const uint32_t*>(Q + (size_t)r * (K / 2) + k0 / 2));
+        s[i] = __ldg(SF + sf_offset(r, k0 / BLOCK, kchunks));
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (r0 + i >= M) break;
+        const float sc = scale_value(s[i]);
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = code_value(w >> (4 * j)) * s;
+        for (int j = 0; j < 4; ++j) {
+            const float2 v = unpack2(w[i] >> (8 * j));
+            f[2 * j] = v.x * sc;
+            f[2 * j + 1] = v.y * sc;
+        }
+        T* dst = Y + (size_t)(r0 + i) * K + k0;
         if constexpr (sizeof(T) == 4) {
-            float4* d = reinterpret_cast<float4*>(Y + i * 8);
-            d[0] = make_float4(f[0], f[1], f[2], f[3]);
-            d[1] = make_float4(f[4], f[5], f[6], f[7]);
+            reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
         } else {
             uint32_t o[4];
 #pragma unroll
@@ -114,14 +199,19 @@ dequant_kernel(const uint8_t* __restrict__ Q, const uint8_t* __restrict__ SF, T*
                 const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
                 o[j] = *reinterpret_cast<const uint32_t*>(&h);
             }
-            *reinterpret_cast<uint4*>(Y + i * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
 }
 
-static int grid_for(uint64_t blocks, const DeviceInfo* info) {
-    const uint64_t most = (uint64_t)info->sm_count * 8;         // 8 CTAs of 256 threads fill an SM
-    return (int)(blocks < most ? (blocks ? blocks : 1) : most);
+// One warp per unit: short-lived CTAs keep every SM's queue of loads full to the
+// end (a resident grid that walked the units took 391 us for 28672x8192 there and
+// back).
+static int grid_for(uint64_t units, const char* name, unsigned* grid) {
+    const uint64_t blocks = (units + THREADS / 32 - 1) / (THREADS / 32);
+    QG_CHECK_ARG(blocks <= INT32_MAX, "%s: tensor is too large", name);
+    *grid = (unsigned)blocks;
+    return QG_OK;
 }
 
 template <typename T>
@@ -129,9 +219,11 @@ static int launch_quant(const void* X, int64_t ldx, void* Q, void* SF, int M, in
     DeviceInfo* info = nullptr;
     int rc = current_device_info(&info);
     if (rc) return rc;
-    const int segs = ((K + ATOM_K - 1) / ATOM_K * ATOM_K + SEG - 1) / SEG;
+    const int width = 32 * Raw<T>::N;
+    const int segs = ((K + ATOM_K - 1) / ATOM_K * ATOM_K + width - 1) / width;
     const uint64_t units = (uint64_t)segs * (uint64_t)((M + 127) / 128 * (128 / ROWS));
-    const int grid = grid_for((units + THREADS / 32 - 1) / (THREADS / 32), info);
+    unsigned grid = 0;
+    if ((rc = grid_for(units, "qg_quant_mxfp4", &grid))) return rc;
     const bool vec = ((uintptr_t)X & 15) == 0 && (ldx * (int64_t)sizeof(T)) % 16 == 0;
     const T* x = static_cast<const T*>(X);
     uint8_t* q = static_cast<uint8_t*>(Q);
@@ -175,7 +267,10 @@ int dequant_mxfp4(const void* Q, const void* SF, void* Y, int out_type, int M, i
     DeviceInfo* info = nullptr;
     int rc = current_device_info(&info);
     if (rc) return rc;
-    const int grid = mx::grid_for(((uint64_t)M * (uint64_t)(K / 8) + mx::THREADS - 1) / mx::THREADS, info);
+    unsigned grid = 0;
+    if ((rc = mx::grid_for((uint64_t)((K + mx::SEG - 1) / mx::SEG) * (uint64_t)((M + mx::ROWS - 1) / mx::ROWS),
+                           "qg_dequant_mxfp4", &grid)))
+        return rc;
     const uint8_t* q = static_cast<const uint8_t*>(Q);
     const uint8_t* sf = static_cast<const uint8_t*>(SF);
     if (out_type == QG_OUT_F32)
