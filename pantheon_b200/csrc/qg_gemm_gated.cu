@@ -5,28 +5,40 @@
 //   backward   dG = dH * U * act'(G), dU = dH * act(G)    (a stream over M x N)
 //              dX = dG Wg + dU Wu                          (contraction over 2 N)
 //              dWg = dG^T X, dWu = dU^T X                  (contraction over M)
+//                                                          (one kernel for the three)
 //
-// All three products are one kernel over CTA pairs (clusters of two, 256 x 256
-// accumulators, tcgen05.mma.cta_group::2 M=256 N=256 K=16 issued by the even
-// CTA; each CTA loads its 128 rows of A and its 128 rows of B per 64-deep
-// block, 32 KB, into a 6-stage ring; two accumulators in TMEM, so a tile's
-// epilogue runs under the next tile's products).  The modes differ in what the
-// operands are:
-//   FWD   A = X; of B's 256 rows the even CTA holds 128 rows of Wg and the odd
-//         CTA the same rows of Wu, so gate and up of an output lie in one TMEM
-//         lane, 128 columns apart, and the epilogue joins them in registers.
-//   DX    A = dG then dU along the contraction; B = Wg then Wu, whose
-//         contraction index is the row: B is read column-major ("MN-major").
-//   DW    A = dG or dU and B = X, both read MN-major: the contraction runs over
-//         the rows of all of them, so nothing is transposed in memory.
-// dG and dU are rounded to the operands' type (the tensor cores take no more):
-// an error of half a step in each, of the size of the output's own rounding.
+// Each product is tiles of CTA pairs (256 x 256 accumulators, tcgen05.mma
+// .cta_group::2 M=256 N=256 K=16 issued by the even CTA); per 64-deep contraction
+// block a CTA loads its 128 rows of A and 128 of B's 256 rows (32 KB) into a
+// 6-stage ring.  TMEM holds two accumulators, tile n of a pair in region n % 2;
+// epilogue group n % 2 drains it under the next tile's products.  (256 x 512
+// tiles, a quarter fewer bytes per product but one accumulator, measured slower:
+// 403 us against 372 forward and 762 against 749 backward at 4096x8192x4096.)
+// What the operands are:
+//   forward   A = X; of B's 256 rows the even CTA holds 128 rows of Wg
+//             and the odd CTA the same rows of Wu, so gate and up of an output lie
+//             in one TMEM lane, 128 columns apart, and the epilogue joins them.
+//   dX        A = dG then dU along the contraction; B = Wg then Wu, whose
+//             contraction index is the row: B is read column-major ("MN-major").
+//   dWg, dWu  A = dG or dU and B = X, both read MN-major: the contraction runs over
+//             the rows of all of them, so nothing is transposed in memory.
+// SPLIT: few tiles share the GPU better when a cluster of S pairs takes one tile
+// and each pair a part of its contraction; the partial tiles meet in shared memory
+// and every CTA joins a share of the columns over distributed shared memory, in
+// rank order (the same bits on every run, no workspace).
+// dG and dU are operands of the tensor cores, so rounded to the type: an error of
+// half a step in each, of the size of the result's own rounding.  Up to 256 rows
+// of X, where few values meet in a sum and the time is that of the weights'
+// bytes, they go as two terms (value and remainder, `parts` = 2): the weights'
+// block is read again from L2 and the rounding is gone.
 // G and U as kept are rounded likewise; H comes from the unrounded sums.
 // All barrier waits are bounded (qg_ptx.cuh).
 #include "qg_common.cuh"
 #include "qg_formats.cuh"
 #include "qg_gated.cuh"
 #include "qg_launch.cuh"
+#include "qg_mxfp4_mma.cuh"
+#include "qg_rows.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,20 +47,26 @@
 namespace qg {
 namespace ffn {
 
+using mx::elect_one;
+using mx::mbar_arrive_relaxed;
+using mx::warp_wait;
+
 enum : int { FWD = 0, DX = 1, DW = 2 };
 
 constexpr int BM = 128;                     // rows of A per CTA
 constexpr int BN = 256;                     // accumulator columns (rows of B per pair)
 constexpr int BK = 64;                      // contraction elements per stage: 128 bytes
 constexpr int UMMA_K = 16;
-constexpr int STAGES = 6;
-constexpr int OP_BYTES = 128 * BK * 2;      // 16 KB: either operand of a CTA
-constexpr int STAGE_BYTES = 2 * OP_BYTES;
+constexpr int OP_BYTES = 128 * BK * 2;      // 16 KB: 128 rows of an operand
 constexpr int MN_BLOCK = 64 * BK * 2;       // 8 KB: 64 columns x 64 contraction rows of an MN-major operand
+constexpr int STAGES = 6;
+constexpr int STAGE_BYTES = 2 * OP_BYTES;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
-constexpr int THREADS = 256;
 constexpr int EPI_WARP0 = 4;
+constexpr int EPI_GROUP = 8;                // epilogue warps of a region: two per TMEM lane quarter
+constexpr int THREADS = (EPI_WARP0 + 2 * EPI_GROUP) * 32;
 constexpr int GROUP_M = 8;                  // row-tiles that share B's tiles in L2 (the bf16 product's best)
+constexpr int MAX_SPLIT = 4;
 
 constexpr uint32_t SITE_PRODUCER = 0x00070001u;
 constexpr uint32_t SITE_MMA_FULL = 0x00070002u;
@@ -65,24 +83,81 @@ struct Barriers {
     int abort;
 };
 
+// Tensor maps: forward X, Wg, Wu; backward also dG and dU with their remainders.
+struct Maps {
+    CUtensorMap x, wg, wu;
+    CUtensorMap rows[2][2]; // [dG, dU][value, remainder] in boxes of 128 rows (dX)
+    CUtensorMap cols[2][2]; // the same in boxes of 64 rows (dWg, dWu)
+};
+
 struct Params {
-    int rows, cols;         // of each output: FWD M x N, DX M x K, DW N x K
-    int k_blocks;           // 64-deep blocks per operand pair (DX: of dG Wg; as many again of dU Wu)
-    int tiles_m, tiles_n;   // DW: the row-tiles of dWg, then those of dWu
-    void* out0;             // H, dX or dWg
-    void* out1;             // G (or null) or dWu
-    void* out2;             // U (or null)
+    int M, N, K;
+    int parts;              // terms of dG and dU (1 or 2)
+    int tiles_dx, tiles_dw; // tiles of dX and of each of dWg, dWu (0: not computed)
+    int tiles;              // in all
+    int ratio;              // see nth_tile
+    void* out0;             // H, or dX
+    void* out1;             // G (or null), or dWg
+    void* out2;             // U (or null), or dWu
     DeviceStatus* status;
 };
 
-__device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& mt, int& nt) {
+// One tile: what it is of, where, and how many 64-deep blocks it sums.
+struct Tile {
+    int kind;               // FWD, DX, DW
+    int which;              // DW: 0 dWg, 1 dWu
+    int mt, nt;
+    int rows, cols;         // of the output
+    int nk;
+};
+
+template <bool BACK>
+__device__ __forceinline__ Tile find_tile(int t, const Params& p) {
+    constexpr int TN = BACK ? BN : BN / 2;                      // output columns of a tile
+    Tile r;
+    if constexpr (!BACK) {
+        r.kind = FWD; r.which = 0; r.rows = p.M; r.cols = p.N; r.nk = (p.K + BK - 1) / BK;
+    } else if (t < p.tiles_dx) {
+        r.kind = DX; r.which = 0; r.rows = p.M; r.cols = p.K; r.nk = 2 * p.parts * ((p.N + BK - 1) / BK);
+    } else {
+        t -= p.tiles_dx;
+        r.kind = DW; r.which = t >= p.tiles_dw; r.rows = p.N; r.cols = p.K; r.nk = p.parts * ((p.M + BK - 1) / BK);
+        if (r.which) t -= p.tiles_dw;
+    }
+    const int tiles_m = (r.rows + 2 * BM - 1) / (2 * BM), tiles_n = (r.cols + TN - 1) / TN;
     const int group = GROUP_M * tiles_n;
     const int g = t / group;
     const int first_m = g * GROUP_M;
     const int gm = min(tiles_m - first_m, GROUP_M);
-    const int r = t - g * group;
-    mt = first_m + r % gm;
-    nt = r / gm;
+    const int q = t - g * group;
+    r.mt = first_m + q % gm;
+    r.nt = q / gm;
+    return r;
+}
+
+// The n-th tile of a pair (p.tiles or more: none).  Tiles go round the pairs; where
+// dX leaves some pairs one of its tiles short, those take as many more tiles of
+// dWg and dWu first (`ratio` = blocks of a dX tile per block of a dW tile).
+template <bool BACK>
+__device__ __forceinline__ int nth_tile(int n, int pair, int pairs, const Params& p) {
+    const int extra = BACK ? p.tiles_dx % pairs : 0;          // pairs with one dX tile more
+    if (extra == 0 || p.tiles_dw == 0) return pair + n * pairs;
+    const int mine = p.tiles_dx / pairs + (pair < extra ? 1 : 0);
+    if (n < mine) return pair + n * pairs;
+    n -= mine;
+    const int others = pairs - extra;
+    if (pair >= extra) {
+        if (n < p.ratio) return p.tiles_dx + (pair - extra) + n * others;
+        n -= p.ratio;
+    }
+    return p.tiles_dx + others * p.ratio + pair + n * pairs;
+}
+
+// Where pair `sub` of `subs` begins in a tile of nk blocks.  A tile of fewer
+// blocks than pairs gives the first nk pairs one each and the others none.
+__device__ __forceinline__ int part_begin(int nk, int sub, int subs) {
+    const int n = min(subs, nk);
+    return sub >= n ? nk : (int)((int64_t)nk * sub / n);
 }
 
 // Descriptor of an MN-major operand tile: blocks of 64 elements (128 bytes)
@@ -97,6 +172,36 @@ __device__ __forceinline__ uint64_t make_sdesc_mnmajor_sw128(uint32_t smem_addr)
     d |= (uint64_t)1u << 46;
     d |= (uint64_t)2u << 61;
     return d;
+}
+
+// 128 rows of an operand: K-major in one box, MN-major in two side by side.
+// Coordinates are in bytes along x (the maps describe byte matrices).
+template <bool MN>
+__device__ __forceinline__ void load_operand(uint8_t* dst, const CUtensorMap* map, uint32_t bar, int row0, int k0) {
+    if constexpr (MN) {
+        tma_load_2d_pair(dst, map, bar, row0 * 2, k0);
+        tma_load_2d_pair(dst + MN_BLOCK, map, bar, row0 * 2 + 128, k0);
+    } else {
+        tma_load_2d_pair(dst, map, bar, k0 * 2, row0);
+    }
+}
+
+// One commit that arrives on the same barrier of both CTAs of a pair.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar, uint32_t pair_in_cluster) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_u32(bar)), "h"((uint16_t)(3u << (2 * pair_in_cluster))) : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_nctas() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
 }
 
 template <typename T> struct Pack;
@@ -119,25 +224,48 @@ template <> struct Pack<__half> {
     }
 };
 
-// 32 values of row `row` from column n0 on; `cols` is a multiple of 8 and rows start on 16 bytes.
 template <typename T>
-__device__ __forceinline__ void store32(void* out, size_t row, int n0, int cols, const float (&f)[32]) {
-    T* dst = static_cast<T*>(out) + row * cols + n0;
+__device__ __forceinline__ void store32(void* out, int row0, const Tile& tl, int n0, const float (&f)[32]) {
+    uint4 v[4];
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-        if (n0 + i < cols)
-            *reinterpret_cast<uint4*>(dst + i) =
-                make_uint4(Pack<T>::two(f[i], f[i + 1]), Pack<T>::two(f[i + 2], f[i + 3]),
-                           Pack<T>::two(f[i + 4], f[i + 5]), Pack<T>::two(f[i + 6], f[i + 7]));
+    for (int i = 0; i < 4; ++i)
+        v[i] = make_uint4(Pack<T>::two(f[8 * i], f[8 * i + 1]), Pack<T>::two(f[8 * i + 2], f[8 * i + 3]),
+                          Pack<T>::two(f[8 * i + 4], f[8 * i + 5]), Pack<T>::two(f[8 * i + 6], f[8 * i + 7]));
+    store_rows(static_cast<uint16_t*>(out), row0, tl.rows, n0, tl.cols, true, v);
 }
 
-template <typename T, int MODE, int ACT>
+// The results of 32 columns (forward: 32 outputs) of the warp's rows row0 + lane.
+template <typename T, bool BACK, int ACT>
+__device__ __forceinline__ void finish32(const Params& p, const Tile& tl, int row0, int n0, const uint32_t (&r0)[32],
+                                         const uint32_t (&r1)[32]) {
+    if (row0 >= tl.rows || n0 >= tl.cols) return;
+    float f[32];
+    if constexpr (BACK) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r0[i]);
+        store32<T>(tl.kind == DX ? p.out0 : tl.which ? p.out2 : p.out1, row0, tl, n0, f);
+    } else {
+        if (p.out1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r0[i]);
+            store32<T>(p.out1, row0, tl, n0, f);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r1[i]);
+            store32<T>(p.out2, row0, tl, n0, f);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = gated<ACT, true>(__uint_as_float(r0[i]), __uint_as_float(r1[i]));
+        store32<T>(p.out0, row0, tl, n0, f);
+    }
+}
+
+template <typename T, bool BACK, int ACT, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
-gated_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
-             const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1, Params p) {
-    constexpr bool A_MN = MODE == DW, B_MN = MODE != FWD;
-    constexpr uint32_t FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    constexpr uint32_t IDESC = make_idesc(1, FMT, FMT, 2 * BM, BN) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+gated_kernel(const __grid_constant__ Maps maps, const Params p) {
+    constexpr int TN = BACK ? BN : BN / 2;                  // output columns of a tile
+    constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t IDESC = make_idesc(1, FMT, FMT, 2 * BM, BN);
+    constexpr uint32_t A_MN = 1u << 15, B_MN = 1u << 16;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -145,26 +273,25 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
     uint8_t* sB = smem + STAGES * OP_BYTES;
     Barriers* bars = reinterpret_cast<Barriers*>(smem + STAGES * STAGE_BYTES);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);   // uniform, and known to be
     const int lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank();
+    const uint32_t crank = cluster_rank();
+    const uint32_t rank = crank & 1u, sub = crank >> 1;     // CTA of the pair, pair of the cluster
+    const uint32_t leader_cta = crank & ~1u;
     const bool leader = rank == 0;
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int half_m = p.tiles_m / 2;                       // DW: where dWu's tiles begin
-    const int nk = MODE == DX ? 2 * p.k_blocks : p.k_blocks;
-    const int pair = blockIdx.x >> 1;
-    const int pairs = gridDim.x >> 1;
+    const int subs = SPLIT ? (int)(cluster_nctas() >> 1) : 1;
+    const int pair = SPLIT ? (int)blockIdx.x / (2 * subs) : (int)blockIdx.x >> 1;
+    const int pairs = SPLIT ? p.tiles : (int)gridDim.x >> 1; // a split cluster has one tile
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(&bars->tmem_full[a], 1); mbar_init(&bars->tmem_empty[a], 8); }
+        for (int a = 0; a < 2; ++a) { mbar_init(&bars->tmem_full[a], 1); mbar_init(&bars->tmem_empty[a], 2 * EPI_GROUP); }
         mbar_init(&bars->drain, 1);
         bars->abort = 0;
         fence_barrier_init();
-        tma_prefetch_desc(&tmA0);
-        tma_prefetch_desc(&tmB0);
-        if (MODE != FWD) tma_prefetch_desc(&tmA1);
-        if (MODE != DW) tma_prefetch_desc(&tmB1);
+        tma_prefetch_desc(&maps.x);
+        tma_prefetch_desc(&maps.wg);
+        tma_prefetch_desc(&maps.wu);
     }
     if (warp == 2) {
         tmem_alloc_pair(&bars->tmem_base, 2 * BN);
@@ -181,34 +308,34 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
         // ------------------------------------------------------------ producer (both CTAs)
         uint32_t stage = 0, phase = 0, armed = 0, armed_phase = 0;
         bool ok = true;
-        for (int t = pair; t < tiles && ok; t += pairs) {
-            int mt, nt;
-            tile_coords(t, p.tiles_m, p.tiles_n, mt, nt);
-            const bool up = MODE == DW && mt >= half_m;      // a tile of dWu
-            const int m0 = (MODE == DW ? mt - (up ? half_m : 0) : mt) * 2 * BM + (int)rank * BM;
-            const int n0 = MODE == FWD ? nt * 128 : nt * BN + (int)rank * 128;
-            for (int kb = 0; kb < nk; ++kb) {
+        for (int n = 0, t; ok && (t = nth_tile<BACK>(n, pair, pairs, p)) < p.tiles; ++n) {
+            const Tile tl = find_tile<BACK>(t, p);
+            const int i0 = SPLIT ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = SPLIT ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
+            const int m0 = tl.mt * 2 * BM + (int)rank * BM;
+            const int nb = (p.N + BK - 1) / BK;
+            for (int i = i0; i < i1; ++i) {
                 if (!mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER)) { ok = false; break; }
                 if (leader) mbar_arrive_expect_tx(&bars->full[stage], 2 * STAGE_BYTES);
-                const uint32_t full = mapa_shared(smem_u32(&bars->full[stage]), 0);
-                const bool second = MODE == DX && kb >= p.k_blocks;   // dU and Wu
-                const int k0 = (second ? kb - p.k_blocks : kb) * BK;
-                const CUtensorMap* a = up || second ? &tmA1 : &tmA0;
-                const CUtensorMap* b = (MODE == FWD && !leader) || second ? &tmB1 : &tmB0;
+                const uint32_t full = mapa_shared(smem_u32(&bars->full[stage]), leader_cta);
                 uint8_t* da = sA + stage * OP_BYTES;
                 uint8_t* db = sB + stage * OP_BYTES;
-                // x coordinates are in bytes (the maps describe byte matrices)
-                if constexpr (A_MN) {
-                    tma_load_2d_pair(da, a, full, m0 * 2, k0);
-                    tma_load_2d_pair(da + MN_BLOCK, a, full, m0 * 2 + 128, k0);
+                if constexpr (!BACK) {
+                    load_operand<false>(da, &maps.x, full, m0, i * BK);
+                    load_operand<false>(db, leader ? &maps.wg : &maps.wu, full, tl.nt * 128, i * BK);
                 } else {
-                    tma_load_2d_pair(da, a, full, k0 * 2, m0);
-                }
-                if constexpr (B_MN) {
-                    tma_load_2d_pair(db, b, full, n0 * 2, k0);
-                    tma_load_2d_pair(db + MN_BLOCK, b, full, n0 * 2 + 128, k0);
-                } else {
-                    tma_load_2d_pair(db, b, full, k0 * 2, n0);
+                    int j = i;
+                    const int part = p.parts == 2 ? (j & 1) : 0;
+                    if (p.parts == 2) j >>= 1;
+                    const CUtensorMap* b = &maps.x;
+                    if (tl.kind == DX) {
+                        const int seg = j >= nb;
+                        if (seg) j -= nb;
+                        b = seg ? &maps.wu : &maps.wg;
+                        load_operand<false>(da, &maps.rows[seg][part], full, m0, j * BK);
+                    } else {
+                        load_operand<true>(da, &maps.cols[tl.which][part], full, m0, j * BK);
+                    }
+                    load_operand<true>(db, b, full, tl.nt * BN + (int)rank * 128, j * BK);
                 }
                 armed |= 1u << stage;
                 armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
@@ -220,107 +347,102 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
             for (int s = 0; s < STAGES; ++s)
                 if (armed & (1u << s)) mbar_wait(&bars->full[s], (armed_phase >> s) & 1u, nullptr, nullptr, 0);
         }
-    } else if (warp == 1 && lane == 0 && leader) {
+    } else if (warp == 1 && leader) {
         // ------------------------------------------------------------ MMA issuer (even CTA)
+        // The whole warp walks the blocks and one elected lane issues: descriptors
+        // and barrier addresses stay in uniform registers.
+        const uint32_t a_addr = smem_u32(sA), b_addr = smem_u32(sB);
         uint32_t stage = 0, phase = 0;
         bool ok = true, issued = false;
-        int iter = 0;
-        for (int t = pair; t < tiles && ok; t += pairs, ++iter) {
-            const uint32_t acc = iter & 1;
-            const uint32_t acc_phase = (iter >> 1) & 1;
-            if (!mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, abort_flag, p.status, SITE_MMA_TMEM)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t d_tmem = tmem_base + acc * BN;
-            for (int kb = 0; kb < nk; ++kb) {
-                if (!mbar_wait(&bars->full[stage], phase, abort_flag, p.status, SITE_MMA_FULL)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t a_addr = smem_u32(sA + stage * OP_BYTES);
-                const uint32_t b_addr = smem_u32(sB + stage * OP_BYTES);
+        int unit = 0;
+        for (int n = 0, t; ok && (t = nth_tile<BACK>(n, pair, pairs, p)) < p.tiles; ++n, ++unit) {
+            const Tile tl = find_tile<BACK>(t, p);
+            const int i0 = SPLIT ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = SPLIT ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
+            auto blocks = [&](auto a_major) {
+                constexpr bool A_IS_MN = decltype(a_major)::value;
+                const uint64_t a_desc = A_IS_MN ? make_sdesc_mnmajor_sw128(a_addr) : make_sdesc_kmajor_sw128(a_addr);
+                const uint64_t b_desc = BACK ? make_sdesc_mnmajor_sw128(b_addr) : make_sdesc_kmajor_sw128(b_addr);
+                // 16 contraction elements: 32 bytes of a K-major row, 16 rows of an MN-major tile
+                constexpr uint32_t A_STEP = A_IS_MN ? UMMA_K * 128 >> 4 : UMMA_K * 2 >> 4;
+                constexpr uint32_t B_STEP = BACK ? UMMA_K * 128 >> 4 : UMMA_K * 2 >> 4;
+                constexpr uint32_t ID = IDESC | (A_IS_MN ? A_MN : 0u) | (BACK ? B_MN : 0u);
+                const uint32_t region = unit & 1, use = unit >> 1;
+                for (int i = i0; i < i1; ++i) {
+                    if (!warp_wait(&bars->full[stage], phase, abort_flag, p.status, SITE_MMA_FULL)) return false;
+                    if (i == i0 && !warp_wait(&bars->tmem_empty[region], (use & 1) ^ 1u, abort_flag, p.status, SITE_MMA_TMEM))
+                        return false;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t ad = a_desc + stage * (OP_BYTES >> 4), bd = b_desc + stage * (OP_BYTES >> 4);
 #pragma unroll
-                for (int k = 0; k < BK / UMMA_K; ++k) {
-                    // 16 contraction elements: 32 bytes of a K-major row, 16 rows of an MN-major tile
-                    const uint64_t ad = A_MN ? make_sdesc_mnmajor_sw128(a_addr + k * UMMA_K * 128)
-                                             : make_sdesc_kmajor_sw128(a_addr + k * UMMA_K * 2);
-                    const uint64_t bd = B_MN ? make_sdesc_mnmajor_sw128(b_addr + k * UMMA_K * 128)
-                                             : make_sdesc_kmajor_sw128(b_addr + k * UMMA_K * 2);
-                    umma_f16_pair(d_tmem, ad, bd, IDESC, (kb | k) != 0 ? 1u : 0u);
+                        for (int k = 0; k < BK / UMMA_K; ++k)
+                            umma_f16_pair(tmem_base + region * BN, ad + k * A_STEP, bd + k * B_STEP, ID,
+                                          i != i0 || k != 0 ? 1u : 0u);
+                        umma_commit_both(&bars->empty[stage], sub);
+                        if (i + 1 == i1) umma_commit_both(&bars->tmem_full[region], sub);
+                    }
+                    __syncwarp();
+                    issued = true;
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
-                issued = true;
-                const uint32_t e = smem_u32(&bars->empty[stage]);
-                umma_commit_pair(mapa_shared(e, 0));
-                umma_commit_pair(mapa_shared(e, 1));
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-            }
-            if (ok) {
-                const uint32_t f = smem_u32(&bars->tmem_full[acc]);
-                umma_commit_pair(mapa_shared(f, 0));
-                umma_commit_pair(mapa_shared(f, 1));
-            }
+                return true;
+            };
+            if (BACK && tl.kind == DW) ok = blocks(std::true_type{});
+            else ok = blocks(std::false_type{});
         }
-        if (!ok && issued) {
-            umma_commit_pair(mapa_shared(smem_u32(&bars->drain), 0));
+        if (!ok && issued && elect_one()) {
+            umma_commit_pair(mapa_shared(smem_u32(&bars->drain), crank));
             mbar_wait(&bars->drain, 0, nullptr, nullptr, 0);
         }
     } else if (warp >= EPI_WARP0) {
         // ------------------------------------------------------------ epilogue (both CTAs)
-        const int ew = warp - EPI_WARP0;
-        int iter = 0;
-        for (int t = pair; t < tiles; t += pairs, ++iter) {
-            int mt, nt;
-            tile_coords(t, p.tiles_m, p.tiles_n, mt, nt);
-            const uint32_t acc = iter & 1;
-            const uint32_t acc_phase = (iter >> 1) & 1;
+        const int group = (warp - EPI_WARP0) / EPI_GROUP;         // tiles group, group + 2, ...
+        const int side = ((warp - EPI_WARP0) % EPI_GROUP) >> 2;   // which half of the columns
+        const int row = (warp & 3) * 32 + lane;
+        const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + group * BN;
+        const uint32_t empty = mapa_shared(smem_u32(&bars->tmem_empty[group]), leader_cta);
+        uint32_t use = 0;
+        for (int unit = group;; unit += 2, ++use) {
+            const int t = nth_tile<BACK>(unit, pair, pairs, p);
+            if (t >= p.tiles) break;
+            const Tile tl = find_tile<BACK>(t, p);
+            const int m_warp = tl.mt * 2 * BM + (int)rank * BM + (warp & 3) * 32;
+            if (SPLIT && ((int)sub >= tl.nk || m_warp >= tl.rows)) break;   // no blocks or no rows: no part
             int ok = 1;
-            if (lane == 0) ok = mbar_wait(&bars->tmem_full[acc], acc_phase, abort_flag, p.status, SITE_EPI) ? 1 : 0;
+            if (lane == 0) ok = mbar_wait(&bars->tmem_full[group], use & 1, abort_flag, p.status, SITE_EPI) ? 1 : 0;
             ok = __shfl_sync(0xffffffffu, ok, 0);
             if (!ok) break;
             tc_fence_after();
-            const bool up = MODE == DW && mt >= half_m;
-            const int m = (MODE == DW ? mt - (up ? half_m : 0) : mt) * 2 * BM + (int)rank * BM + ew * 32 + lane;
-            const bool row_ok = m < p.rows;
-            const uint32_t t_row = tmem_base + ((uint32_t)(ew * 32) << 16) + acc * BN;
-            if constexpr (MODE == FWD) {
+            if constexpr (SPLIT) {
+                // this pair's part of the sums, column by column over the drained ring
+                float* part = reinterpret_cast<float*>(smem) + row;
 #pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t rg[32], ru[32];
-                    __syncwarp();
-                    tmem_ld_32x32b_x32(t_row + c, rg);
-                    tmem_ld_32x32b_x32(t_row + 128 + c, ru);
-                    tmem_ld_wait_regs(rg);
-                    tmem_ld_wait_regs(ru);
-                    const int n0 = nt * 128 + c;
-                    if (!row_ok || n0 >= p.cols) continue;
-                    float f[32];
-                    if (p.out1) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(rg[i]);
-                        store32<T>(p.out1, m, n0, p.cols, f);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(ru[i]);
-                        store32<T>(p.out2, m, n0, p.cols, f);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) f[i] = gated<ACT, true>(__uint_as_float(rg[i]), __uint_as_float(ru[i]));
-                    store32<T>(p.out0, m, n0, p.cols, f);
-                }
-            } else {
-#pragma unroll 1
-                for (int c = 0; c < BN; c += 32) {
+                for (int c = side * (BN / 2); c < (side + 1) * (BN / 2); c += 32) {
                     uint32_t r[32];
                     __syncwarp();
                     tmem_ld_32x32b_x32(t_row + c, r);
                     tmem_ld_wait_regs(r);
-                    const int n0 = nt * BN + c;
-                    if (!row_ok || n0 >= p.cols) continue;
-                    float f[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
-                    store32<T>(up ? p.out1 : p.out0, m, n0, p.cols, f);
+                    for (int i = 0; i < 32; ++i) part[(c + i) * BM] = __uint_as_float(r[i]);
+                }
+            } else {
+#pragma unroll 1
+                for (int c = side * (TN / 2); c < (side + 1) * (TN / 2); c += 32) {
+                    uint32_t r0[32], r1[32];
+                    __syncwarp();
+                    tmem_ld_32x32b_x32(t_row + c, r0);
+                    if constexpr (!BACK) tmem_ld_32x32b_x32(t_row + BN / 2 + c, r1);
+                    tmem_ld_wait_regs(r0);
+                    if constexpr (!BACK) tmem_ld_wait_regs(r1);
+                    if (c + 32 == (side + 1) * (TN / 2)) {
+                        // the warp's last columns are in registers: the region may be overwritten
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_relaxed(empty);
+                    }
+                    finish32<T, BACK, ACT>(p, tl, m_warp, tl.nt * TN + c, r0, r1);
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars->tmem_empty[acc]), 0));
         }
     }
 
@@ -333,32 +455,68 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ C
         tmem_dealloc_pair(tmem_base, 2 * BN);
         if (lane == 0 && *abort_flag) atomicAdd(&p.status->drained, 1u);
     }
+    if constexpr (SPLIT) {
+        // every CTA joins its share of the columns, 32 at a time, from the same CTA of each pair
+        if (warp >= EPI_WARP0) {
+            const Tile tl = find_tile<BACK>(pair, p);
+            const int row = (warp & 3) * 32 + lane;
+            const int m_warp = tl.mt * 2 * BM + (int)rank * BM + (warp & 3) * 32;
+            const uint32_t base = smem_u32(smem) + (uint32_t)row * 4;
+            const int c_end = m_warp < tl.rows ? TN : 0;        // (no rows in this warp: nothing)
+            for (int c = ((int)sub + subs * ((warp - EPI_WARP0) >> 2)) * 32; c < c_end; c += subs * 4 * 32) {
+                uint32_t r0[32] = {}, r1[32] = {};               // fp32 zeros
+                for (int k = 0; k < min(subs, tl.nk); ++k) {
+                    const uint32_t at = mapa_shared(base + (uint32_t)(c * BM) * 4, 2u * k + rank);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        r0[i] = __float_as_uint(__uint_as_float(r0[i]) + ld_cluster_f32(at + i * BM * 4));
+                        if constexpr (!BACK)
+                            r1[i] = __float_as_uint(__uint_as_float(r1[i]) + ld_cluster_f32(at + (BN / 2 + i) * BM * 4));
+                    }
+                }
+                finish32<T, BACK, ACT>(p, tl, m_warp, tl.nt * TN + c, r0, r1);
+            }
+        }
+        cluster_sync();                                           // nobody leaves while its part is being read
+    }
 }
 
-// dG = dH * U * act'(G), dU = dH * act(G), eight elements per thread and step.
-// Five streams of 2 bytes per element: bound by memory.
-template <typename T, int ACT>
+// dG = dH * U * act'(G), dU = dH * act(G), eight elements per thread, in `parts`
+// terms (the value rounded to T, and what that left out).  Five streams of
+// 2 bytes per element: bound by memory.
+template <typename T, int ACT, int PARTS>
 __global__ void __launch_bounds__(256)
 gate_backward_kernel(const uint4* __restrict__ dH, const uint4* __restrict__ G, const uint4* __restrict__ U,
-                     uint4* __restrict__ dG, uint4* __restrict__ dU, uint64_t n8) {
-    const uint64_t step = (uint64_t)gridDim.x * blockDim.x;
+                     uint4* __restrict__ D, uint64_t n8) {
     wait_previous_grid();
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += step) {
-        const uint4 vh = __ldg(dH + i), vg = __ldg(G + i), vu = __ldg(U + i);
-        const uint32_t h[4] = {vh.x, vh.y, vh.z, vh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
-        uint32_t og[4], ou[4];
+    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n8) return;
+    const uint4 vh = __ldg(dH + i), vg = __ldg(G + i), vu = __ldg(U + i);
+    const uint32_t h[4] = {vh.x, vh.y, vh.z, vh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
+    uint32_t o[2][2][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 fh = Pack<T>::unpack(h[j]), fg = Pack<T>::unpack(g[j]), fu = Pack<T>::unpack(u[j]);
-            float a0, s0, a1, s1;
-            gate_slope<ACT>(fg.x, a0, s0);
-            gate_slope<ACT>(fg.y, a1, s1);
-            og[j] = Pack<T>::two(fh.x * fu.x * s0, fh.y * fu.y * s1);
-            ou[j] = Pack<T>::two(fh.x * a0, fh.y * a1);
+    for (int j = 0; j < 4; ++j) {
+        const float2 fh = Pack<T>::unpack(h[j]), fg = Pack<T>::unpack(g[j]), fu = Pack<T>::unpack(u[j]);
+        float a0, s0, a1, s1;
+        gate_slope<ACT>(fg.x, a0, s0);
+        gate_slope<ACT>(fg.y, a1, s1);
+        const float d[2][2] = {{fh.x * fu.x * s0, fh.y * fu.y * s1}, {fh.x * a0, fh.y * a1}};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            o[w][0][j] = Pack<T>::two(d[w][0], d[w][1]);
+            if constexpr (PARTS == 2) {
+                const float2 r = Pack<T>::unpack(o[w][0][j]);
+                // (a value past the type's range has no remainder: infinity stays infinity)
+                o[w][1][j] = Pack<T>::two(isinf(r.x) ? 0.0f : d[w][0] - r.x, isinf(r.y) ? 0.0f : d[w][1] - r.y);
+            }
         }
-        dG[i] = make_uint4(og[0], og[1], og[2], og[3]);
-        dU[i] = make_uint4(ou[0], ou[1], ou[2], ou[3]);
     }
+    // D: dG, dU, then their remainders, n8 words each
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+            D[(uint64_t)(2 * q + w) * n8 + i] = make_uint4(o[w][q][0], o[w][q][1], o[w][q][2], o[w][q][3]);
 }
 
 // The byte matrix of a 2-byte tensor [rows, cols] in boxes of 128 bytes x box_rows.
@@ -367,38 +525,72 @@ static int make_map(CUtensorMap* map, const void* base, int rows, int cols, int 
                         (uint64_t)cols * 2, 128, (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int MODE, int ACT>
-static int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0, const CUtensorMap& b1, Params p,
-                  cudaStream_t stream) {
-    DeviceInfo* info = nullptr;
-    int rc = current_device_info(&info);
-    if (rc) return rc;
-    if ((rc = device_status_ptr(&p.status))) return rc;
-    QG_CUDA(cudaFuncSetAttribute(gated_kernel<T, MODE, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
-    // persistent pairs: as many as can be resident at once
-    static int resident[64] = {};
+// Clusters of `ctas` CTAs that can be resident at once (they need free SMs of one
+// GPC, so this can be below sm_count / ctas).  All forms of the kernel have the
+// same block and shared-memory size, so `kernel` stands for all of them.
+static int resident_clusters(void (*kernel)(Maps, Params), int ctas, int* out, const DeviceInfo* info) {
+    static int known[64][2 * MAX_SPLIT + 1] = {};
     int dev = 0;
     QG_CUDA(cudaGetDevice(&dev));
-    int res = resident[dev & 63];
+    int& res = known[dev & 63][ctas];
     if (!res) {
+        QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
         cudaLaunchConfig_t lc = {};
-        lc.gridDim = dim3(info->sm_count & ~1);
+        lc.gridDim = dim3(info->sm_count / ctas * ctas);
         lc.blockDim = dim3(THREADS);
         lc.dynamicSmemBytes = SMEM_BYTES;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim = {2, 1, 1};
+        at[0].val.clusterDim = {(unsigned)ctas, 1, 1};
         lc.attrs = at;
         lc.numAttrs = 1;
-        QG_CUDA(cudaOccupancyMaxActiveClusters(&res, gated_kernel<T, MODE, ACT>, &lc));
-        if (res < 1) res = 1;
-        resident[dev & 63] = res;
+        int n = 0;
+        QG_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &lc));
+        res = n > 0 ? n : 1;
     }
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int pairs = tiles < res ? tiles : res;
-    QG_CUDA(launch_overlapped(gated_kernel<T, MODE, ACT>, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, 2, a0, a1, b0,
-                              b1, p));
+    *out = res;
     return QG_OK;
+}
+
+template <typename T, bool BACK, int ACT, bool SPLIT>
+static int launch_kernel(const Maps& maps, Params p, int subs, const DeviceInfo* info, cudaStream_t stream) {
+    constexpr int TN = BACK ? BN : BN / 2;
+    if constexpr (!BACK) p.tiles = ceil_div(p.M, 2 * BM) * ceil_div(p.N, TN);
+    else {
+        if (p.tiles_dx) p.tiles_dx = ceil_div(p.M, 2 * BM) * ceil_div(p.K, TN);
+        if (p.tiles_dw) p.tiles_dw = ceil_div(p.N, 2 * BM) * ceil_div(p.K, TN);
+        p.tiles = p.tiles_dx + 2 * p.tiles_dw;
+    }
+    auto kernel = gated_kernel<T, BACK, ACT, SPLIT>;
+    QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+    int pairs = 0;
+    if constexpr (SPLIT) pairs = p.tiles * subs;
+    else {
+        int rc = resident_clusters(kernel, 2, &pairs, info);
+        if (rc) return rc;
+        if (p.tiles < pairs) pairs = p.tiles;
+    }
+    QG_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, 2 * subs, maps, p));
+    return QG_OK;
+}
+
+// Which form, of `units` tiles and `nk` blocks in the longest: a cluster of 2 or 4
+// pairs per tile while all of them fit at once and the longest gives each two
+// blocks; otherwise a pair per tile.
+template <typename T, bool BACK, int ACT>
+static int launch(const Maps& maps, Params p, int64_t units, int nk, cudaStream_t stream) {
+    DeviceInfo* info = nullptr;
+    int rc = current_device_info(&info);
+    if (rc) return rc;
+    if ((rc = device_status_ptr(&p.status))) return rc;
+    int subs = 1;
+    for (int s = 2; s <= MAX_SPLIT && 2 * s <= nk; s *= 2) {
+        int clusters = 0;
+        if ((rc = resident_clusters(gated_kernel<T, BACK, ACT, true>, 2 * s, &clusters, info))) return rc;
+        if (units <= clusters) subs = s;
+    }
+    return subs > 1 ? launch_kernel<T, BACK, ACT, true>(maps, p, subs, info, stream)
+                    : launch_kernel<T, BACK, ACT, false>(maps, p, 1, info, stream);
 }
 
 static int check_shape(const char* name, int M, int N, int K) {
@@ -407,9 +599,12 @@ static int check_shape(const char* name, int M, int N, int K) {
     // x coordinates are bytes in 32 bits; tile counts fit too
     QG_CHECK_ARG(M <= (1 << 29) && N <= (1 << 29) && K <= (1 << 29), "%s: shape %dx%dx%d is too large", name, M, N, K);
     const int64_t m = ceil_div(M, 256), n = ceil_div(N, 128), k = ceil_div(K, 256);
-    QG_CHECK_ARG(m * n <= (1 << 30) && m * k <= (1 << 30) && n * k <= (1 << 30), "%s: shape %dx%dx%d is too large", name, M, N, K);
+    QG_CHECK_ARG(m * n <= (1 << 29) && m * k <= (1 << 29) && n * k <= (1 << 29), "%s: shape %dx%dx%d is too large", name, M, N, K);
     return QG_OK;
 }
+
+// Terms of dG and dU (see the head of this file).
+static int grad_parts(int M) { return M <= 2 * BM ? 2 : 1; }
 
 template <typename T>
 static int forward(const char* name, const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, int act,
@@ -421,12 +616,15 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
     if (rc) return rc;
     QG_CHECK_ARG((((uintptr_t)X | (uintptr_t)Wg | (uintptr_t)Wu | (uintptr_t)H | (uintptr_t)G | (uintptr_t)U) & 15) == 0,
                  "%s: operands and outputs must be 16-byte aligned", name);
-    CUtensorMap a, b0, b1;
-    if ((rc = make_map(&a, X, M, K, BM)) || (rc = make_map(&b0, Wg, N, K, 128)) || (rc = make_map(&b1, Wu, N, K, 128)))
+    Maps maps;
+    if ((rc = make_map(&maps.x, X, M, K, BM)) || (rc = make_map(&maps.wg, Wg, N, K, 128)) ||
+        (rc = make_map(&maps.wu, Wu, N, K, 128)))
         return rc;
-    Params p{M, N, ceil_div(K, BK), ceil_div(M, 2 * BM), ceil_div(N, 128), H, G, U, nullptr};
-    return act == QG_ACT_SILU ? launch<T, FWD, QG_ACT_SILU>(a, a, b0, b1, p, stream)
-                              : launch<T, FWD, QG_ACT_GELU_TANH>(a, a, b0, b1, p, stream);
+    for (int i = 0; i < 4; ++i) maps.rows[i >> 1][i & 1] = maps.cols[i >> 1][i & 1] = maps.x;   // not read
+    const Params p{M, N, K, 1, 0, 0, 0, 0, H, G, U, nullptr};
+    const int64_t units = (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN / 2);
+    return act == QG_ACT_SILU ? launch<T, false, QG_ACT_SILU>(maps, p, units, ceil_div(K, BK), stream)
+                              : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
 }
 
 template <typename T>
@@ -439,41 +637,54 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     QG_CHECK_ARG(act == QG_ACT_SILU || act == QG_ACT_GELU_TANH, "%s: unknown activation %d", name, act);
     int rc = check_shape(name, M, N, K);
     if (rc) return rc;
+    const int parts = grad_parts(M);
     const uint64_t one = (uint64_t)M * (uint64_t)N * 2;           // a multiple of 16
-    QG_CHECK_ARG(workspace && workspace_bytes >= 2 * one, "%s: workspace of %llu bytes, %llu needed", name,
-                 (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)(2 * one));
+    QG_CHECK_ARG(workspace && workspace_bytes >= 2 * parts * one, "%s: workspace of %llu bytes, %llu needed", name,
+                 (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)(2 * parts * one));
     QG_CHECK_ARG((((uintptr_t)dH | (uintptr_t)X | (uintptr_t)Wg | (uintptr_t)Wu | (uintptr_t)G | (uintptr_t)U |
                    (uintptr_t)dX | (uintptr_t)dWg | (uintptr_t)dWu | (uintptr_t)workspace) & 15) == 0,
                  "%s: operands, outputs and workspace must be 16-byte aligned", name);
     DeviceInfo* info = nullptr;
     if ((rc = current_device_info(&info))) return rc;
-    void* dG = workspace;
-    void* dU = static_cast<uint8_t*>(workspace) + one;
-    const uint64_t n8 = one / 16, blocks = (n8 + 255) / 256, most = (uint64_t)info->sm_count * 8;
-    const int grid = (int)(blocks < most ? blocks : most);
+    const uint64_t n8 = one / 16, blocks = (n8 + 255) / 256;
+    QG_CHECK_ARG(blocks <= INT32_MAX, "%s: shape %dx%d is too large", name, M, N);
     auto* vh = static_cast<const uint4*>(dH);
     auto* vg = static_cast<const uint4*>(G);
     auto* vu = static_cast<const uint4*>(U);
-    auto* og = static_cast<uint4*>(dG);
-    auto* ou = static_cast<uint4*>(dU);
-    QG_CUDA(launch_overlapped(act == QG_ACT_SILU ? gate_backward_kernel<T, QG_ACT_SILU>
-                                                 : gate_backward_kernel<T, QG_ACT_GELU_TANH>,
-                              dim3(grid), dim3(256), 0, stream, 1, vh, vg, vu, og, ou, n8));
-    CUtensorMap a0, a1, b0, b1;
-    if (dX) {
-        if ((rc = make_map(&a0, dG, M, N, BM)) || (rc = make_map(&a1, dU, M, N, BM)) ||
-            (rc = make_map(&b0, Wg, N, K, BK)) || (rc = make_map(&b1, Wu, N, K, BK)))
-            return rc;
-        Params p{M, K, ceil_div(N, BK), ceil_div(M, 2 * BM), ceil_div(K, BN), dX, nullptr, nullptr, nullptr};
-        if ((rc = launch<T, DX, QG_ACT_SILU>(a0, a1, b0, b1, p, stream))) return rc;
+    const bool silu = act == QG_ACT_SILU;
+    auto kernel = parts == 2 ? (silu ? gate_backward_kernel<T, QG_ACT_SILU, 2> : gate_backward_kernel<T, QG_ACT_GELU_TANH, 2>)
+                             : (silu ? gate_backward_kernel<T, QG_ACT_SILU, 1> : gate_backward_kernel<T, QG_ACT_GELU_TANH, 1>);
+    QG_CUDA(launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, 1, vh, vg, vu,
+                              static_cast<uint4*>(workspace), n8));
+    Maps maps;
+    for (int w = 0; w < 2; ++w)
+        for (int q = 0; q < 2; ++q) {
+            // (without remainders their maps are not read)
+            void* d = static_cast<uint8_t*>(workspace) + (2 * (q < parts ? q : 0) + w) * one;
+            if ((rc = make_map(&maps.rows[w][q], d, M, N, BM)) || (rc = make_map(&maps.cols[w][q], d, M, N, BK))) return rc;
+        }
+    if ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)) || (rc = make_map(&maps.x, X, M, K, BK)))
+        return rc;
+    const int nk_dx = 2 * parts * ceil_div(N, BK), nk_dw = parts * ceil_div(M, BK);
+    const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
+    const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
+    const Params p{M, N, K, parts, 0, 0, 0, (nk_dx + nk_dw / 2) / nk_dw, dX, dWg, dWu, nullptr};
+    // dX alone when it has few tiles (few rows of X): it is split then, and dWg and
+    // dWu are not.  Otherwise the three share one launch, whichever are asked for: the
+    // same split, so the same bits.
+    if (4 * units_dx <= info->sm_count) {
+        Params q = p;
+        q.tiles_dx = 1;
+        if (dX && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_dx, nk_dx, stream))) return rc;
+        q = p;
+        q.tiles_dw = 1;
+        if (dWg && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_dw, nk_dw, stream))) return rc;
+        return QG_OK;
     }
-    if (dWg) {
-        if ((rc = make_map(&a0, dG, M, N, BK)) || (rc = make_map(&a1, dU, M, N, BK)) || (rc = make_map(&b0, X, M, K, BK)))
-            return rc;
-        Params p{N, K, ceil_div(M, BK), 2 * ceil_div(N, 2 * BM), ceil_div(K, BN), dWg, dWu, nullptr, nullptr};
-        if ((rc = launch<T, DW, QG_ACT_SILU>(a0, a1, b0, b0, p, stream))) return rc;
-    }
-    return QG_OK;
+    Params q = p;
+    q.tiles_dx = dX ? 1 : 0;
+    q.tiles_dw = dWg ? 1 : 0;
+    return launch<T, true, QG_ACT_SILU>(maps, q, units_dx + units_dw, nk_dx > nk_dw ? nk_dx : nk_dw, stream);
 }
 
 } // namespace ffn
@@ -493,7 +704,7 @@ extern "C" int qg_gemm_gated_f16(const void* X, const void* Wg, const void* Wu, 
 
 extern "C" int qg_gemm_gated_backward_workspace_bytes(int M, int N, uint64_t* bytes) {
     QG_CHECK_ARG(bytes && M > 0 && N > 0, "qg_gemm_gated_backward_workspace_bytes: bad argument");
-    *bytes = 4ull * (uint64_t)M * (uint64_t)N;
+    *bytes = 4ull * (uint64_t)qg::ffn::grad_parts(M) * (uint64_t)M * (uint64_t)N;
     return QG_OK;
 }
 

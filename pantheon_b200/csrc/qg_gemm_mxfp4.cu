@@ -31,6 +31,7 @@
 #include "qg_launch.cuh"
 #include "qg_mxfp4.cuh"
 #include "qg_mxfp4_mma.cuh"
+#include "qg_rows.cuh"
 
 #include <cuda_bf16.h>
 
@@ -103,38 +104,28 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
     nt = r / gm;
 }
 
-// Store COLS values of one output row from column n0 on (columns past N are left out).
-template <int OUT, int COLS>
-__device__ __forceinline__ void store_row(void* C, size_t row, int n0, int N, bool vec, const float (&f)[COLS]) {
+// 32 values of each of the warp's rows row0 + lane, from column n0 on.
+template <int OUT>
+__device__ __forceinline__ void store32(const GemmParams& p, int row0, int n0, const float (&f)[32]) {
+    if (row0 >= p.M || n0 >= p.N) return;
     if constexpr (OUT == QG_OUT_F32) {
-        float* dst = static_cast<float*>(C) + row * N + n0;
-        if (vec && n0 + COLS <= N) {
+        uint4 v[8];
 #pragma unroll
-            for (int i = 0; i < COLS; i += 4)
-                *reinterpret_cast<float4*>(dst + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < COLS; ++i)
-                if (n0 + i < N) dst[i] = f[i];
-        }
+        for (int i = 0; i < 8; ++i)
+            v[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
+                              __float_as_uint(f[4 * i + 3]));
+        store_rows(static_cast<uint32_t*>(p.C), row0, p.M, n0, p.N, p.vec, v);
     } else {
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(C) + row * N + n0;
-        if (vec && n0 + COLS <= N) {
+        uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < COLS; i += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(f[i + 2 * j], f[i + 2 * j + 1]);
-                    w[j] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-                *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < COLS; ++i)
-                if (n0 + i < N) dst[i] = __float2bfloat16_rn(f[i]);
+        for (int i = 0; i < 16; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        store_rows(static_cast<uint16_t*>(p.C), row0, p.M, n0, p.N, p.vec, v);
     }
 }
 
@@ -197,7 +188,6 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, uint64_t* tmem_ful
     const int tiles = tiles_m * tiles_n;
     const int quarter = warp & 3;
     const int part = (warp - EPI_WARP0) >> 2;             // which quarter of the columns
-    const int row = quarter * 32 + lane;
     // gated: 32 gate columns and the 32 up columns of the same outputs
     const uint32_t c0 = GATED ? part * 32 : part * 64;
     const uint32_t c1 = GATED ? BN / 2 + part * 32 : part * 64 + 32;
@@ -224,17 +214,17 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, uint64_t* tmem_ful
         __syncwarp();
         if (lane == 0) mbar_arrive_relaxed(tmem_empty);     // orders TMEM reads only
 
-        const int m = mt * tile_rows + row0 + row;
+        const int m_warp = mt * tile_rows + row0 + quarter * 32;
+        const int m = m_warp + lane;
         if constexpr (!GATED) {
-            if (m >= p.M) continue;
             const int n0 = nt * BN + part * 64;
             float f[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r0[i]);
-            if (n0 < p.N) store_row<OUT, 32>(p.C, m, n0, p.N, p.vec, f);
+            store32<OUT>(p, m_warp, n0, f);
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r1[i]);
-            if (n0 + 32 < p.N) store_row<OUT, 32>(p.C, m, n0 + 32, p.N, p.vec, f);
+            store32<OUT>(p, m_warp, n0 + 32, f);
         } else {
             const int n0 = nt * TN + part * 32;
             float f[32];
@@ -265,7 +255,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, uint64_t* tmem_ful
                 // zero past M and N in the atoms' padding (a pair's odd CTA may lie past that too)
                 if (m < out_rows) p.SFC[sf_offset(m, j, out_kchunks)] = (uint8_t)s;
             } else {
-                if (m < p.M && n0 < p.N) store_row<OUT, 32>(p.C, m, n0, p.N, p.vec, f);
+                store32<OUT>(p, m_warp, n0, f);
             }
         }
     }

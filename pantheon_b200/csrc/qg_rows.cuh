@@ -1,0 +1,64 @@
+// qg_rows.cuh -- stores of accumulator rows.  An epilogue warp has a row per lane
+// (TMEM's layout), so a lane's 16-byte stores meet 31 other rows in one
+// instruction: 32 lines, a clock each.  Exchanged among four (eight) neighbouring
+// lanes first, each instruction writes 64 (128) contiguous bytes of eight (four)
+// rows instead.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace qg {
+
+__device__ __forceinline__ uint4 shfl_xor_u4(uint4 v, int mask) {
+    return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, mask), __shfl_xor_sync(0xffffffffu, v.y, mask),
+                      __shfl_xor_sync(0xffffffffu, v.z, mask), __shfl_xor_sync(0xffffffffu, v.w, mask));
+}
+
+// N x N transpose of 16-byte pieces among groups of N neighbouring lanes: v[j] of
+// lane q becomes what was v[q] of lane j.  The whole warp calls it.
+template <int N>
+__device__ __forceinline__ void transpose_lanes(uint4 (&v)[N]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int m = 1; m < N; m *= 2) {
+        const bool high = lane & m;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if ((i & m) == 0) {
+                const uint4 got = shfl_xor_u4(high ? v[i] : v[i + m], m);
+                if (high) v[i] = got;
+                else v[i + m] = got;
+            }
+    }
+}
+
+// The warp's 32 rows x 16 N bytes (lane l: row l): rows row0 + l below `rows`, from
+// element `n0` (of `elem` bytes) on of rows of `cols` elements.  `vec`: rows and
+// n0 start on 16 bytes and cols is a multiple of 16 bytes.  The whole warp calls it.
+template <typename E, int N>
+__device__ __forceinline__ void store_rows(E* out, int row0, int rows, int n0, int cols, bool vec, uint4 (&v)[N]) {
+    constexpr int PER = 16 / sizeof(E);
+    transpose_lanes(v);
+    const int lane = threadIdx.x & 31;
+    const int n = n0 + (lane % N) * PER;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int r = row0 + (lane & ~(N - 1)) + j;
+        if (r >= rows || n >= cols) continue;
+        E* dst = out + (size_t)r * cols + n;
+        if (vec) {
+            *reinterpret_cast<uint4*>(dst) = v[j];
+        } else {
+            const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (n + i < cols) {
+                    if constexpr (sizeof(E) == 4) dst[i] = w[i];
+                    else dst[i] = (E)(w[i / 2] >> (16 * (i & 1)));
+                }
+        }
+    }
+}
+
+} // namespace qg

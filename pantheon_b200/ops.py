@@ -332,7 +332,7 @@ def _gemm_gated_backward(entry: str, dtype: torch.dtype, dH, X, Wg, Wu, G, U, ac
     dWg = torch.empty((N, K), dtype=dtype, device=X.device) if need_dw else None
     dWu = torch.empty((N, K), dtype=dtype, device=X.device) if need_dw else None
     if workspace is None:
-        workspace = torch.empty((4 * M * N,), dtype=torch.uint8, device=X.device)
+        workspace = torch.empty((gemm_gated_backward_workspace_bytes(M, N),), dtype=torch.uint8, device=X.device)
     else:
         _require(f"{entry}: workspace", workspace, torch.uint8, tuple(workspace.shape), X)
     _launch(entry, X, dH, X, Wg, Wu, G, U, dX, dWg, dWu, act, M, N, K, workspace, workspace.numel())
@@ -364,7 +364,7 @@ def gemm_gated_bf16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor
                              U: torch.Tensor, act: int = QG_ACT_SILU, need_dx: bool = True, need_dw: bool = True,
                              workspace: torch.Tensor | None = None):
     """Gradients (dX, dWg, dWu) of gemm_gated_bf16 from dH [M,N] and the G, U it kept; a gradient
-    that is not needed is None.  dG and dU are rounded to bf16 on the way.  `workspace` (uint8,
+    that is not needed is None.  Above 256 rows dG and dU are rounded to bf16 on the way.  `workspace` (uint8,
     gemm_gated_backward_workspace_bytes) is allocated when not given."""
     return _gemm_gated_backward("qg_gemm_gated_bf16_backward", torch.bfloat16, dH, X, Wg, Wu, G, U, act, need_dx,
                                 need_dw, workspace)
