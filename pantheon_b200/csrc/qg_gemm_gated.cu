@@ -574,9 +574,24 @@ static int launch_kernel(const Maps& maps, Params p, int subs, const DeviceInfo*
     return QG_OK;
 }
 
-// Which form, of `units` tiles and `nk` blocks in the longest: a cluster of 2 or 4
-// pairs per tile while all of them fit at once and the longest gives each two
-// blocks; otherwise a pair per tile.
+// Pairs per tile, of `units` tiles and `nk` blocks in the longest: 4 or 2 while all
+// the clusters fit at once and the contraction is long enough.  Joining the parts
+// costs about 4.5 us (128 KB per CTA over distributed shared memory), a block
+// 0.3 us: with 16 blocks a split loses (1x1024x1024 9.8 us against 8.9), with 32 and
+// more it wins (256x2048x2048 14.5 against 17.1, 64x1024x4096 14.9 against 24.0).
+constexpr int SPLIT_MIN_BLOCKS = 20;
+template <typename T, bool BACK, int ACT>
+static int pick_split(int* out, int64_t units, int nk, const DeviceInfo* info) {
+    *out = 1;
+    for (int s = 2; s <= MAX_SPLIT && nk >= SPLIT_MIN_BLOCKS; s *= 2) {
+        int clusters = 0;
+        const int rc = resident_clusters(gated_kernel<T, BACK, ACT, true>, 2 * s, &clusters, info);
+        if (rc) return rc;
+        if (units <= clusters) *out = s;
+    }
+    return QG_OK;
+}
+
 template <typename T, bool BACK, int ACT>
 static int launch(const Maps& maps, Params p, int64_t units, int nk, cudaStream_t stream) {
     DeviceInfo* info = nullptr;
@@ -584,11 +599,7 @@ static int launch(const Maps& maps, Params p, int64_t units, int nk, cudaStream_
     if (rc) return rc;
     if ((rc = device_status_ptr(&p.status))) return rc;
     int subs = 1;
-    for (int s = 2; s <= MAX_SPLIT && 2 * s <= nk; s *= 2) {
-        int clusters = 0;
-        if ((rc = resident_clusters(gated_kernel<T, BACK, ACT, true>, 2 * s, &clusters, info))) return rc;
-        if (units <= clusters) subs = s;
-    }
+    if ((rc = pick_split<T, BACK, ACT>(&subs, units, nk, info))) return rc;
     return subs > 1 ? launch_kernel<T, BACK, ACT, true>(maps, p, subs, info, stream)
                     : launch_kernel<T, BACK, ACT, false>(maps, p, 1, info, stream);
 }
@@ -669,10 +680,15 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
     const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
     const Params p{M, N, K, parts, 0, 0, 0, (nk_dx + nk_dw / 2) / nk_dw, dX, dWg, dWu, nullptr};
-    // dX alone when it has few tiles (few rows of X): it is split then, and dWg and
-    // dWu are not.  Otherwise the three share one launch, whichever are asked for: the
-    // same split, so the same bits.
-    if (4 * units_dx <= info->sm_count) {
+    // One launch for the three, unless dX is the long pole: few tiles (few rows of X)
+    // of many blocks, which a launch of its own splits, beside many of few blocks.
+    // (Decided for all three, whichever are asked for: the same split, the same bits.)
+    const int nk = nk_dx > nk_dw ? nk_dx : nk_dw;
+    int all = 1, alone = 1;
+    if ((rc = pick_split<T, true, QG_ACT_SILU>(&all, units_dx + units_dw, nk, info)) ||
+        (rc = pick_split<T, true, QG_ACT_SILU>(&alone, units_dx, nk_dx, info)))
+        return rc;
+    if (all == 1 && alone > 1 && nk_dx > 2 * nk_dw) {
         Params q = p;
         q.tiles_dx = 1;
         if (dX && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_dx, nk_dx, stream))) return rc;
@@ -684,7 +700,7 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     Params q = p;
     q.tiles_dx = dX ? 1 : 0;
     q.tiles_dw = dWg ? 1 : 0;
-    return launch<T, true, QG_ACT_SILU>(maps, q, units_dx + units_dw, nk_dx > nk_dw ? nk_dx : nk_dw, stream);
+    return launch<T, true, QG_ACT_SILU>(maps, q, units_dx + units_dw, nk, stream);
 }
 
 } // namespace ffn
