@@ -235,8 +235,8 @@ def quant_mxfp4(X: torch.Tensor):
         raise ValueError("quant_mxfp4: the last dimension must be contiguous")
     if M > 1 and X.stride(0) < K:
         raise ValueError(f"quant_mxfp4: rows must not overlap (row stride {X.stride(0)} < K={K})")
-    sf = torch.empty((mxfp4_sf_bytes(M, K),), dtype=torch.uint8, device=X.device)
-    q = torch.empty((M, (K + 31) // 32 * 16), dtype=torch.uint8, device=X.device)
+    sf = X.new_empty((mxfp4_sf_bytes(M, K),), dtype=torch.uint8)
+    q = X.new_empty((M, (K + 31) // 32 * 16), dtype=torch.uint8)
     _launch("qg_quant_mxfp4", X, X, _MX_IN_TYPES[X.dtype], X.stride(0) if M > 1 else K, q, sf, M, K)
     return q, sf
 
@@ -256,7 +256,7 @@ def dequant_mxfp4(Q: torch.Tensor, SF: torch.Tensor, out_type: int = QG_OUT_BF16
     M, K = _mx_operand("dequant_mxfp4: Q", Q, SF, Q)
     if out_type not in (QG_OUT_BF16, QG_OUT_F32):
         raise ValueError(f"dequant_mxfp4: out_type {out_type} (bf16 or f32)")
-    out = torch.empty((M, K), dtype=_OUT_DTYPES[out_type], device=Q.device)
+    out = Q.new_empty((M, K), dtype=_OUT_DTYPES[out_type])
     _launch("qg_dequant_mxfp4", Q, Q, SF, out, out_type, M, K)
     return out
 
@@ -274,7 +274,7 @@ def gemm_mxfp4(A: torch.Tensor, sfa: torch.Tensor, B: torch.Tensor, sfb: torch.T
     if out_type not in (QG_OUT_BF16, QG_OUT_F32):
         raise ValueError(f"gemm_mxfp4: out_type {out_type} (bf16 or f32)")
     if out is None:
-        out = torch.empty((M, N), dtype=_OUT_DTYPES[out_type], device=A.device)
+        out = A.new_empty((M, N), dtype=_OUT_DTYPES[out_type])
     else:
         _require("gemm_mxfp4: out", out, _OUT_DTYPES[out_type], (M, N), A)
     _launch("qg_gemm_mxfp4", A, A, sfa, B, sfb, out, out_type, M, N, K)
@@ -296,10 +296,10 @@ def gemm_gated_mxfp4(A: torch.Tensor, sfa: torch.Tensor, Wg: torch.Tensor, sfg: 
     if out_type == QG_OUT_MXFP4:
         if N % 32:
             raise ValueError(f"gemm_gated_mxfp4: N={N} must be a multiple of 32 for an MXFP4 result")
-        out = torch.empty((M, N // 2), dtype=torch.uint8, device=A.device)
-        sfh = torch.empty((mxfp4_sf_bytes(M, N),), dtype=torch.uint8, device=A.device)
+        out = A.new_empty((M, N // 2))
+        sfh = A.new_empty((mxfp4_sf_bytes(M, N),))
     elif out_type in (QG_OUT_BF16, QG_OUT_F32):
-        out = torch.empty((M, N), dtype=_OUT_DTYPES[out_type], device=A.device)
+        out = A.new_empty((M, N), dtype=_OUT_DTYPES[out_type])
     else:
         raise ValueError(f"gemm_gated_mxfp4: out_type {out_type} (bf16, f32 or mxfp4)")
     _launch("qg_gemm_gated_mxfp4", A, A, sfa, Wg, sfg, Wu, sfu, out, sfh, out_type, act, M, N, K)
@@ -319,22 +319,22 @@ def _gated_shape(entry: str, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor
 
 def _gemm_gated(entry: str, dtype: torch.dtype, X, Wg, Wu, act, keep):
     M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
-    out = [torch.empty((M, N), dtype=dtype, device=X.device) for _ in range(3 if keep else 1)]
-    _launch(entry, X, X, Wg, Wu, out[0], out[1] if keep else None, out[2] if keep else None, act, M, N, K)
-    return tuple(out) if keep else out[0]
+    H = X.new_empty((M, N))
+    G, U = (torch.empty_like(H), torch.empty_like(H)) if keep else (None, None)
+    _launch(entry, X, X, Wg, Wu, H, G, U, act, M, N, K)
+    return (H, G, U) if keep else H
 
 
 def _gemm_gated_backward(entry: str, dtype: torch.dtype, dH, X, Wg, Wu, G, U, act, need_dx, need_dw, workspace):
     M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
     for name, t in (("dH", dH), ("G", G), ("U", U)):
         _require(f"{entry}: {name}", t, dtype, (M, N), X)
-    dX = torch.empty((M, K), dtype=dtype, device=X.device) if need_dx else None
-    dWg = torch.empty((N, K), dtype=dtype, device=X.device) if need_dw else None
-    dWu = torch.empty((N, K), dtype=dtype, device=X.device) if need_dw else None
+    dX = torch.empty_like(X) if need_dx else None
+    dWg, dWu = (torch.empty_like(Wg), torch.empty_like(Wu)) if need_dw else (None, None)
     if workspace is None:
-        workspace = torch.empty((gemm_gated_backward_workspace_bytes(M, N),), dtype=torch.uint8, device=X.device)
+        workspace = X.new_empty((gemm_gated_backward_workspace_bytes(M, N),), dtype=torch.uint8)
     else:
-        _require(f"{entry}: workspace", workspace, torch.uint8, tuple(workspace.shape), X)
+        _require(f"{entry}: workspace", workspace, torch.uint8, workspace.shape, X)
     _launch(entry, X, dH, X, Wg, Wu, G, U, dX, dWg, dWu, act, M, N, K, workspace, workspace.numel())
     return dX, dWg, dWu
 
