@@ -757,7 +757,9 @@ static int check_mx(const char* name, const void* A, const void* SFA, const void
     QG_CHECK_ARG(A && SFA && B && SFB && C, "%s: null operand or output", name);
     QG_CHECK_ARG(M > 0 && N > 0 && K > 0, "%s: empty shape %dx%dx%d", name, M, N, K);
     QG_CHECK_ARG(K % 32 == 0, "%s: K=%d must be a multiple of 32", name, K);
-    QG_CHECK_ARG((int64_t)ceil_div(M, BM) * ceil_div(N, BN / 2) <= INT32_MAX / 2, "%s: shape %dx%d is too large", name, M, N);
+    QG_CHECK_ARG(M <= (1 << 30) && N <= (1 << 30) && K <= (1 << 30) &&
+                     (int64_t)ceil_div(M, BM) * ceil_div(N, BN / 2) <= (1 << 30),
+                 "%s: shape %dx%dx%d is too large", name, M, N, K);
     QG_CHECK_ARG((((uintptr_t)A | (uintptr_t)SFA | (uintptr_t)B | (uintptr_t)SFB) & 15) == 0,
                  "%s: codes and scales must be 16-byte aligned", name);
     return QG_OK;

@@ -98,6 +98,47 @@ def test_backward_matches_the_formula(cuda_device, shape, act, kind):
     assert pb.device_status(0) == 0
 
 
+# several tiles per CTA pair (forward 96 tiles; backward 165 tiles of two lengths), dX split alone
+# beside whole dWg and dWu, and two-term gradients at their limit of 256 rows
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", [(700, 4000, 136), (1100, 1032, 2600), (100, 5000, 256), (256, 512, 776), (257, 512, 776)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_larger_shapes(cuda_device, shape, kind):
+    x, wg, wu = _inputs(shape, kind, cuda_device)
+    forward, backward = TYPES[kind][3:]
+    act = ACTS[shape[0] % 2]
+    h, g, u = forward(x, wg, wu, act=act, keep=True)
+    _check_forward(x, wg, wu, act, kind, h, g, u)
+    dh = torch.randn(g.shape, device=cuda_device, generator=torch.Generator(cuda_device).manual_seed(6)).to(g.dtype)
+    got = backward(dh, x, wg, wu, g, u, act=act)
+    _check_backward(dh, x, wg, wu, g, u, act, kind, got)
+    assert torch.equal(backward(dh, x, wg, wu, g, u, act=act, need_dw=False)[0], got[0])
+    assert torch.equal(backward(dh, x, wg, wu, g, u, act=act, need_dx=False)[2], got[2])
+    assert pb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_few_rows_carry_no_intermediate_rounding(cuda_device, kind):
+    """Up to 256 rows dG and dU go as value and remainder: what is left of their rounding is a
+    half step of the remainder, so the results are within their own rounding and the fp32 bounds."""
+    M, N, K = 48, 264, 136
+    x, wg, wu = _inputs((M, N, K), kind, cuda_device)
+    forward, backward, step = TYPES[kind][3], TYPES[kind][4], TYPES[kind][1]
+    _, g, u = forward(x, wg, wu, keep=True)
+    dh = torch.randn(g.shape, device=cuda_device, generator=torch.Generator(cuda_device).manual_seed(7)).to(g.dtype)
+    dx, dwg, dwu = (_np(t) for t in backward(dh, x, wg, wu, g, u))
+    dh, x, wg, wu, g, u = (_np(t) for t in (dh, x, wg, wu, g, u))
+    dg, du = dh * u * R.slope(g, 0), dh * R.activation(g, 0)
+    # fp32 gradients: 40 units with |g| of a few (checked below); remainder: step^2, or fp16's least half step
+    assert np.abs(g).max() < 16
+    rel, least = 200 * 2.0 ** -23 + step * step, TYPES[kind][2]
+    edg, edu = rel * (np.abs(dh * u) + np.abs(dg)) + least, rel * (np.abs(dh) * (1 + np.abs(g)) + np.abs(du)) + least
+    for have, ref, e in ((dx, dg @ wg + du @ wu, edg @ np.abs(wg) + edu @ np.abs(wu) + 4 * R.sum_bound(np.abs(dg), wg.T) + 4 * R.sum_bound(np.abs(du), wu.T)),
+                         (dwg, dg.T @ x, edg.T @ np.abs(x) + 2 * R.sum_bound(dg.T, x.T)),
+                         (dwu, du.T @ x, edu.T @ np.abs(x) + 2 * R.sum_bound(du.T, x.T))):
+        assert (np.abs(have - ref) <= e + _half_step(np.abs(ref) + e, kind)).all()
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_backward_against_differences(cuda_device, act):
     """Central differences of the 64-bit forward pass.  X and the weights are small multiples of 1/2,

@@ -138,6 +138,46 @@ def test_gated_matches_the_definition(cuda_device, shape, act):
     assert pb.device_status(0) == 0
 
 
+# one shape for each kernel beyond the few-rows one: single CTAs (more than 64, gated 32, rows with
+# tiles for half of the SMs), CTA pairs (more than 128 rows), and pairs with several tiles each
+WIDE = [(70, 19001, 288), (130, 10001, 544), (200, 5024, 1056), (513, 9999, 96), (1400, 4320, 800)]
+
+
+@pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32])
+@pytest.mark.parametrize("shape", WIDE, ids=lambda s: "x".join(map(str, s)))
+def test_wide_gemm_matches_the_definition(cuda_device, shape, out_type):
+    M, N, K = shape
+    a, av = _operand(M, K, M + K, cuda_device)
+    b, bv = _operand(N, K, N + 3 * K, cuda_device)
+    ref, e = av @ bv.T, R.sum_bound(av, bv)
+    y = _np(pb.gemm_mxfp4(*a, *b, out_type=out_type))
+    assert (np.abs(y - ref) <= e + (2.0 ** -8 * np.abs(ref) if out_type == pb.QG_OUT_BF16 else 0)).all()
+    assert pb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32, pb.QG_OUT_MXFP4])
+@pytest.mark.parametrize("shape", [(40, 9601, 288), (64, 9632, 352), (130, 5001, 544), (200, 4928, 1056), (513, 5024, 96),
+                                   (1400, 2176, 416)], ids=lambda s: "x".join(map(str, s)))
+def test_wide_gated_matches_the_definition(cuda_device, shape, out_type):
+    M, N, K = shape
+    if out_type == pb.QG_OUT_MXFP4 and N % 32:
+        N += 32 - N % 32
+    act = ACTS[M % 2]
+    a, av = _operand(M, K, M + K, cuda_device)
+    g, gv = _operand(N, K, N + 3 * K, cuda_device)
+    u, uv = _operand(N, K, N + 5 * K, cuda_device)
+    gate, up = av @ gv.T, av @ uv.T
+    with np.errstate(over="ignore"):
+        ref = R.activation(gate, act) * up
+        e = R.gated_bound(gate, up, R.sum_bound(av, gv), R.sum_bound(av, uv), act)
+    y = pb.gemm_gated_mxfp4(*a, *g, *u, act=act, out_type=out_type)
+    if out_type == pb.QG_OUT_MXFP4:
+        _check_mx_result(_np(y[0]), _np(y[1]), ref, e)
+    else:
+        assert (np.abs(_np(y) - ref) <= e + (2.0 ** -8 * np.abs(ref) if out_type == pb.QG_OUT_BF16 else 0)).all()
+    assert pb.device_status(0) == 0
+
+
 def _check_mx_result(q, sf, ref, e):
     """The conversion of values within e of ref: scales by the block's maximum, values by half a step."""
     M, N = ref.shape
@@ -265,3 +305,32 @@ def test_python_refusals(cuda_device):
         pb.quant_mxfp4(torch.zeros((0, 64), device=cuda_device))
     with pytest.raises(ValueError):
         pb.dequant_mxfp4(q, sf, pb.QG_OUT_F16)
+
+
+def test_first_calls_of_a_process_can_be_captured(cuda_device):
+    """Every operator's first call inside a stream capture, in a process of its own."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+import pantheon_b200 as pb
+x = torch.randn((200, 256), device="cuda").to(torch.bfloat16)
+w = torch.randn((5024, 256), device="cuda").to(torch.bfloat16) / 16
+torch.cuda.synchronize()
+def run():
+    q, p = pb.quant_mxfp4(x), pb.quant_mxfp4(w)
+    h, g, u = pb.gemm_gated_bf16(x, w, w, keep=True)
+    return (pb.dequant_mxfp4(*q), pb.gemm_mxfp4(*q, *p), pb.gemm_mxfp4(*p, *q), pb.gemm_gated_mxfp4(*q, *p, *p), h,
+            *pb.gemm_gated_bf16_backward(h, x, w, w, g, u))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, run()))
+print("captured")
+"""
+    root = Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
