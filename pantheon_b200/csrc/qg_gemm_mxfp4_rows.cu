@@ -393,12 +393,13 @@ static int launch(const void* X, const void* W, const void* W2, const Params& p,
     const int nk = (p.K + BK - 1) / BK;
     const int nt = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
     const int64_t tiles = (int64_t)ceil_div(p.N, ACT >= 0 ? BW / 2 : BW) * ceil_div(p.M, nt);
-    // As many CTAs as one wave holds (two per SM), two K blocks each at least: a
-    // CTA's start and end cost 2-3 us, which a second wave pays again.  Measured
-    // (K=8192, one row): N=28672 22.8 us unsplit, 26.1 in two, 31.5 in four;
-    // N=8192 14.1, 10.7, 10.4 and 13.9 in eight; N=1024 13.3, 8.6, 6.2, 5.1.
+    // As many CTAs as one wave holds (two per SM), four K blocks each at least: a
+    // CTA's start and end cost 2-3 us, which a second wave pays again, and the join
+    // grows with the split.  Measured (one row, K=8192): N=28672 22.8 us unsplit, 26.1
+    // in two, 31.5 in four; N=8192 14.1, 10.7, 10.4 and 13.9 in eight; N=1024 13.3, 8.6,
+    // 6.2, 5.1.  333 x 1001 x 4128 (17 blocks): 7.4 in four, 9.6 in eight.
     int split = 1;
-    while (split < 8 && 2 * split * tiles <= 2 * info->sm_count && 4 * split <= nk) split *= 2;
+    while (split < 8 && 2 * split * tiles <= 2 * info->sm_count && 8 * split <= nk) split *= 2;
     switch (nt) {
         case 16: return launch_nt<16, OUT, ACT>(X, W, W2, p, split, stream);
         case 32: return launch_nt<32, OUT, ACT>(X, W, W2, p, split, stream);
