@@ -138,8 +138,10 @@ __device__ __forceinline__ Tile find_tile(int t, const Params& p) {
 // The n-th tile of a pair (p.tiles or more: none).  Tiles go round the pairs; where
 // dX leaves some pairs one of its tiles short, those take as many more tiles of
 // dWg and dWu first (`ratio` = blocks of a dX tile per block of a dW tile).
-template <bool BACK>
+// A split cluster has the one tile of its number.
+template <bool BACK, bool SPLIT>
 __device__ __forceinline__ int nth_tile(int n, int pair, int pairs, const Params& p) {
+    if (SPLIT) return n == 0 ? pair : p.tiles;
     const int extra = BACK ? p.tiles_dx % pairs : 0;          // pairs with one dX tile more
     if (extra == 0 || p.tiles_dw == 0) return pair + n * pairs;
     const int mine = p.tiles_dx / pairs + (pair < extra ? 1 : 0);
@@ -281,7 +283,7 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
     const bool leader = rank == 0;
     const int subs = SPLIT ? (int)(cluster_nctas() >> 1) : 1;
     const int pair = SPLIT ? (int)blockIdx.x / (2 * subs) : (int)blockIdx.x >> 1;
-    const int pairs = SPLIT ? p.tiles : (int)gridDim.x >> 1; // a split cluster has one tile
+    const int pairs = (int)gridDim.x >> 1;                  // (not of use to a split cluster)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
@@ -308,7 +310,7 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
         // ------------------------------------------------------------ producer (both CTAs)
         uint32_t stage = 0, phase = 0, armed = 0, armed_phase = 0;
         bool ok = true;
-        for (int n = 0, t; ok && (t = nth_tile<BACK>(n, pair, pairs, p)) < p.tiles; ++n) {
+        for (int n = 0, t; ok && (t = nth_tile<BACK, SPLIT>(n, pair, pairs, p)) < p.tiles; ++n) {
             const Tile tl = find_tile<BACK>(t, p);
             const int i0 = SPLIT ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = SPLIT ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
             const int m0 = tl.mt * 2 * BM + (int)rank * BM;
@@ -355,7 +357,7 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
         uint32_t stage = 0, phase = 0;
         bool ok = true, issued = false;
         int unit = 0;
-        for (int n = 0, t; ok && (t = nth_tile<BACK>(n, pair, pairs, p)) < p.tiles; ++n, ++unit) {
+        for (int n = 0, t; ok && (t = nth_tile<BACK, SPLIT>(n, pair, pairs, p)) < p.tiles; ++n, ++unit) {
             const Tile tl = find_tile<BACK>(t, p);
             const int i0 = SPLIT ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = SPLIT ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
             auto blocks = [&](auto a_major) {
@@ -403,15 +405,12 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
         const uint32_t empty = mapa_shared(smem_u32(&bars->tmem_empty[group]), leader_cta);
         uint32_t use = 0;
         for (int unit = group;; unit += 2, ++use) {
-            const int t = nth_tile<BACK>(unit, pair, pairs, p);
+            const int t = nth_tile<BACK, SPLIT>(unit, pair, pairs, p);
             if (t >= p.tiles) break;
             const Tile tl = find_tile<BACK>(t, p);
             const int m_warp = tl.mt * 2 * BM + (int)rank * BM + (warp & 3) * 32;
             if (SPLIT && ((int)sub >= tl.nk || m_warp >= tl.rows)) break;   // no blocks or no rows: no part
-            int ok = 1;
-            if (lane == 0) ok = mbar_wait(&bars->tmem_full[group], use & 1, abort_flag, p.status, SITE_EPI) ? 1 : 0;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok) break;
+            if (!warp_wait(&bars->tmem_full[group], use & 1, abort_flag, p.status, SITE_EPI)) break;
             tc_fence_after();
             if constexpr (SPLIT) {
                 // this pair's part of the sums, column by column over the drained ring

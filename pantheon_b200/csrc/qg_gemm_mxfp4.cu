@@ -199,10 +199,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& p, uint64_t* tmem_ful
     for (int t = first; t < tiles; t += step, ++iter) {
         int mt, nt;
         tile_coords(t, tiles_m, tiles_n, p.group_m, mt, nt);
-        int ok = 1;
-        if (lane == 0) ok = mbar_wait(tmem_full, iter & 1, abort_flag, p.status, SITE_EPI) ? 1 : 0;
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
+        if (!warp_wait(tmem_full, iter & 1, abort_flag, p.status, SITE_EPI)) break;
         tc_fence_after();
         uint32_t r0[32], r1[32];
         __syncwarp();

@@ -249,10 +249,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUt
             if (++stage == G::STAGES) { stage = 0; phase ^= 1u; }
         }
         // ------------------------------------------------------------ the partial tile
-        int done = 0;
-        if (ok && lane == 0) done = mbar_wait(&bars->acc_full, 0, abort_flag, p.status, SITE_EPI) ? 1 : 0;
-        done = __shfl_sync(0xffffffffu, done, 0);
-        if (done) {
+        if (ok && warp_wait(&bars->acc_full, 0, abort_flag, p.status, SITE_EPI)) {
             tc_fence_after();
             float* dst = part + quarter * 32 + lane;
 #pragma unroll
