@@ -667,12 +667,16 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     QG_CUDA(launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, 1, vh, vg, vu,
                               static_cast<uint4*>(workspace), n8));
     Maps maps;
-    for (int w = 0; w < 2; ++w)
-        for (int q = 0; q < 2; ++q) {
-            // (without remainders their maps are not read)
-            void* d = static_cast<uint8_t*>(workspace) + (2 * (q < parts ? q : 0) + w) * one;
+    for (int w = 0; w < 2; ++w) {
+        for (int q = 0; q < parts; ++q) {
+            void* d = static_cast<uint8_t*>(workspace) + (2 * q + w) * one;
             if ((rc = make_map(&maps.rows[w][q], d, M, N, BM)) || (rc = make_map(&maps.cols[w][q], d, M, N, BK))) return rc;
         }
+        if (parts == 1) {               // not read
+            maps.rows[w][1] = maps.rows[w][0];
+            maps.cols[w][1] = maps.cols[w][0];
+        }
+    }
     if ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)) || (rc = make_map(&maps.x, X, M, K, BK)))
         return rc;
     const int nk_dx = 2 * parts * ceil_div(N, BK), nk_dw = parts * ceil_div(M, BK);

@@ -186,27 +186,31 @@ def gen_nvfp4(M: int, N: int, K: int, seed: int, tid0: int = 0, device="cuda"):
     return A, sfa, B, sfb, g
 
 
-def _launch(entry: str, like: torch.Tensor, *args):
-    """A C entry on like's device and that device's current stream; tensors go as their addresses."""
+def _launch(entry: str, device: int, *args):
+    """A C entry on `device` and its current stream; args are numbers and addresses."""
     fn = getattr(load_library(), entry)
-    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
-    index = like.get_device()
-    stream = torch._C._cuda_getCurrentRawStream(index)   # current_stream(index).cuda_stream, without its object
-    if index == torch.cuda.current_device():
+    stream = torch._C._cuda_getCurrentRawStream(device)   # current_stream(device).cuda_stream, without its object
+    if device == torch.cuda.current_device():
         code = fn(*args, stream)
     else:   # a launch goes to the current device
-        with torch.cuda.device(index):
+        with torch.cuda.device(device):
             code = fn(*args, stream)
     if code:
         check(entry, code)
 
 
-def _require(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, like: torch.Tensor):
-    """A contiguous CUDA tensor of this type and shape on like's device."""
-    if t.dtype is dtype and t.shape == shape and t.is_cuda and t.get_device() == like.get_device() and t.is_contiguous():
+def _require(entry: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int):
+    """A contiguous CUDA tensor of this type and shape on the device."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
         return
     _require_cuda(t)
-    raise ValueError(f"{name} must be {dtype} {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    raise ValueError(f"{entry}: {name} must be {dtype} {list(shape)} on cuda:{device}, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _device_of(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError("pantheon_b200 kernels take CUDA tensors only (no CPU fallback)")
+    return t.get_device()
 
 
 _MX_IN_TYPES = {torch.bfloat16: QG_OUT_BF16, torch.float16: QG_OUT_F16, torch.float32: QG_OUT_F32}
@@ -226,38 +230,40 @@ def quant_mxfp4(X: torch.Tensor):
     scales uint8 ue8m0 in the atom layout (see include/pantheon_qgemm.h).  A block of 32 that holds
     a NaN or an infinity becomes NaN.  Asynchronous on the current stream.
     """
-    if not X.is_cuda:
-        raise ValueError("pantheon_b200 kernels take CUDA tensors only (no CPU fallback)")
-    if X.dim() != 2 or X.dtype not in _MX_IN_TYPES:
+    device = _device_of(X)
+    in_type = _MX_IN_TYPES.get(X.dtype)
+    if X.dim() != 2 or in_type is None:
         raise ValueError(f"quant_mxfp4: a 2-D bf16, fp16 or fp32 tensor, got {X.dtype} {list(X.shape)}")
     M, K = X.shape
-    if K > 1 and X.stride(1) != 1:
+    row, col = X.stride()
+    if K > 1 and col != 1:
         raise ValueError("quant_mxfp4: the last dimension must be contiguous")
-    if M > 1 and X.stride(0) < K:
-        raise ValueError(f"quant_mxfp4: rows must not overlap (row stride {X.stride(0)} < K={K})")
+    if M > 1 and row < K:
+        raise ValueError(f"quant_mxfp4: rows must not overlap (row stride {row} < K={K})")
     sf = X.new_empty((mxfp4_sf_bytes(M, K),), dtype=torch.uint8)
     q = X.new_empty((M, (K + 31) // 32 * 16), dtype=torch.uint8)
-    _launch("qg_quant_mxfp4", X, X, _MX_IN_TYPES[X.dtype], X.stride(0) if M > 1 else K, q, sf, M, K)
+    _launch("qg_quant_mxfp4", device, X.data_ptr(), in_type, row if M > 1 else K, q.data_ptr(), sf.data_ptr(), M, K)
     return q, sf
 
 
-def _mx_operand(name: str, Q: torch.Tensor, SF: torch.Tensor, like: torch.Tensor):
+def _mx_operand(entry: str, name: str, Q: torch.Tensor, SF: torch.Tensor, device: int):
     """(rows, K) of an MXFP4 operand."""
     if Q.dim() != 2:
-        raise ValueError(f"{name}: codes must be 2-D, got {list(Q.shape)}")
+        raise ValueError(f"{entry}: {name} codes must be 2-D, got {list(Q.shape)}")
     rows, half = Q.shape
-    _require(name, Q, torch.uint8, (rows, half), like)
-    _require(name, SF, torch.uint8, (mxfp4_sf_bytes(rows, 2 * half),), like)
+    _require(entry, name, Q, torch.uint8, (rows, half), device)
+    _require(entry, name, SF, torch.uint8, (mxfp4_sf_bytes(rows, 2 * half),), device)
     return rows, 2 * half
 
 
 def dequant_mxfp4(Q: torch.Tensor, SF: torch.Tensor, out_type: int = QG_OUT_BF16) -> torch.Tensor:
     """The values an MXFP4 tensor stands for, [M, K] bf16 or fp32 (both exact)."""
-    M, K = _mx_operand("dequant_mxfp4: Q", Q, SF, Q)
+    device = _device_of(Q)
+    M, K = _mx_operand("dequant_mxfp4", "Q", Q, SF, device)
     if out_type not in (QG_OUT_BF16, QG_OUT_F32):
         raise ValueError(f"dequant_mxfp4: out_type {out_type} (bf16 or f32)")
     out = Q.new_empty((M, K), dtype=_OUT_DTYPES[out_type])
-    _launch("qg_dequant_mxfp4", Q, Q, SF, out, out_type, M, K)
+    _launch("qg_dequant_mxfp4", device, Q.data_ptr(), SF.data_ptr(), out.data_ptr(), out_type, M, K)
     return out
 
 
@@ -267,8 +273,9 @@ def gemm_mxfp4(A: torch.Tensor, sfa: torch.Tensor, B: torch.Tensor, sfb: torch.T
 
     fp32 accumulation on the tensor cores; any M and N, K % 32 == 0 (what quant_mxfp4 gives).
     """
-    M, K = _mx_operand("gemm_mxfp4: A", A, sfa, A)
-    N, K2 = _mx_operand("gemm_mxfp4: B", B, sfb, A)
+    device = _device_of(A)
+    M, K = _mx_operand("gemm_mxfp4", "A", A, sfa, device)
+    N, K2 = _mx_operand("gemm_mxfp4", "B", B, sfb, device)
     if K != K2:
         raise ValueError(f"K mismatch {K} vs {K2}")
     if out_type not in (QG_OUT_BF16, QG_OUT_F32):
@@ -276,8 +283,9 @@ def gemm_mxfp4(A: torch.Tensor, sfa: torch.Tensor, B: torch.Tensor, sfb: torch.T
     if out is None:
         out = A.new_empty((M, N), dtype=_OUT_DTYPES[out_type])
     else:
-        _require("gemm_mxfp4: out", out, _OUT_DTYPES[out_type], (M, N), A)
-    _launch("qg_gemm_mxfp4", A, A, sfa, B, sfb, out, out_type, M, N, K)
+        _require("gemm_mxfp4", "out", out, _OUT_DTYPES[out_type], (M, N), device)
+    _launch("qg_gemm_mxfp4", device, A.data_ptr(), sfa.data_ptr(), B.data_ptr(), sfb.data_ptr(), out.data_ptr(), out_type,
+            M, N, K)
     return out
 
 
@@ -288,9 +296,10 @@ def gemm_gated_mxfp4(A: torch.Tensor, sfa: torch.Tensor, Wg: torch.Tensor, sfg: 
     out_type QG_OUT_BF16 or QG_OUT_F32 gives H [M, N]; QG_OUT_MXFP4 (N % 32 == 0) gives (codes,
     scales), the A operand of the down projection.
     """
-    M, K = _mx_operand("gemm_gated_mxfp4: A", A, sfa, A)
-    N, K2 = _mx_operand("gemm_gated_mxfp4: Wg", Wg, sfg, A)
-    if _mx_operand("gemm_gated_mxfp4: Wu", Wu, sfu, A) != (N, K2) or K != K2:
+    device = _device_of(A)
+    M, K = _mx_operand("gemm_gated_mxfp4", "A", A, sfa, device)
+    N, K2 = _mx_operand("gemm_gated_mxfp4", "Wg", Wg, sfg, device)
+    if _mx_operand("gemm_gated_mxfp4", "Wu", Wu, sfu, device) != (N, K2) or K != K2:
         raise ValueError(f"gemm_gated_mxfp4: A {list(A.shape)}, Wg {list(Wg.shape)} and Wu {list(Wu.shape)} do not match")
     sfh = None
     if out_type == QG_OUT_MXFP4:
@@ -302,40 +311,47 @@ def gemm_gated_mxfp4(A: torch.Tensor, sfa: torch.Tensor, Wg: torch.Tensor, sfg: 
         out = A.new_empty((M, N), dtype=_OUT_DTYPES[out_type])
     else:
         raise ValueError(f"gemm_gated_mxfp4: out_type {out_type} (bf16, f32 or mxfp4)")
-    _launch("qg_gemm_gated_mxfp4", A, A, sfa, Wg, sfg, Wu, sfu, out, sfh, out_type, act, M, N, K)
+    _launch("qg_gemm_gated_mxfp4", device, A.data_ptr(), sfa.data_ptr(), Wg.data_ptr(), sfg.data_ptr(), Wu.data_ptr(),
+            sfu.data_ptr(), out.data_ptr(), sfh.data_ptr() if sfh is not None else None, out_type, act, M, N, K)
     return (out, sfh) if out_type == QG_OUT_MXFP4 else out
 
 
 def _gated_shape(entry: str, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, dtype: torch.dtype):
+    """(device, M, N, K) of a gated product's operands."""
+    device = _device_of(X)
     if X.dim() != 2 or Wg.dim() != 2:
         raise ValueError(f"{entry}: X and Wg must be 2-D")
     M, K = X.shape
     N = Wg.shape[0]
-    _require(f"{entry}: X", X, dtype, (M, K), X)
-    _require(f"{entry}: Wg", Wg, dtype, (N, K), X)
-    _require(f"{entry}: Wu", Wu, dtype, (N, K), X)
-    return M, N, K
+    _require(entry, "X", X, dtype, (M, K), device)
+    _require(entry, "Wg", Wg, dtype, (N, K), device)
+    _require(entry, "Wu", Wu, dtype, (N, K), device)
+    return device, M, N, K
 
 
 def _gemm_gated(entry: str, dtype: torch.dtype, X, Wg, Wu, act, keep):
-    M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
+    device, M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
     H = X.new_empty((M, N))
     G, U = (torch.empty_like(H), torch.empty_like(H)) if keep else (None, None)
-    _launch(entry, X, X, Wg, Wu, H, G, U, act, M, N, K)
+    _launch(entry, device, X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), H.data_ptr(), G.data_ptr() if keep else None,
+            U.data_ptr() if keep else None, act, M, N, K)
     return (H, G, U) if keep else H
 
 
 def _gemm_gated_backward(entry: str, dtype: torch.dtype, dH, X, Wg, Wu, G, U, act, need_dx, need_dw, workspace):
-    M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
-    for name, t in (("dH", dH), ("G", G), ("U", U)):
-        _require(f"{entry}: {name}", t, dtype, (M, N), X)
+    device, M, N, K = _gated_shape(entry, X, Wg, Wu, dtype)
+    _require(entry, "dH", dH, dtype, (M, N), device)
+    _require(entry, "G", G, dtype, (M, N), device)
+    _require(entry, "U", U, dtype, (M, N), device)
     dX = torch.empty_like(X) if need_dx else None
     dWg, dWu = (torch.empty_like(Wg), torch.empty_like(Wu)) if need_dw else (None, None)
     if workspace is None:
         workspace = X.new_empty((gemm_gated_backward_workspace_bytes(M, N),), dtype=torch.uint8)
     else:
-        _require(f"{entry}: workspace", workspace, torch.uint8, workspace.shape, X)
-    _launch(entry, X, dH, X, Wg, Wu, G, U, dX, dWg, dWu, act, M, N, K, workspace, workspace.numel())
+        _require(entry, "workspace", workspace, torch.uint8, workspace.shape, device)
+    _launch(entry, device, dH.data_ptr(), X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), G.data_ptr(), U.data_ptr(),
+            dX.data_ptr() if need_dx else None, dWg.data_ptr() if need_dw else None, dWu.data_ptr() if need_dw else None,
+            act, M, N, K, workspace.data_ptr(), workspace.numel())
     return dX, dWg, dWu
 
 
