@@ -63,9 +63,13 @@ constexpr int STAGES = 6;
 constexpr int STAGE_BYTES = 2 * OP_BYTES;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
 constexpr int EPI_WARP0 = 4;
-constexpr int EPI_GROUP = 8;                // epilogue warps of a region: two per TMEM lane quarter
+constexpr int EPI_GROUP = 4;                // epilogue warps of a region, one per TMEM lane quarter (two: 368 us against 350)
 constexpr int THREADS = (EPI_WARP0 + 2 * EPI_GROUP) * 32;
-constexpr int GROUP_M = 8;                  // row-tiles that share B's tiles in L2 (the bf16 product's best)
+// Row-tiles that share B's tiles in L2 before the next columns: backward 8 (4 and
+// 16 within 1 % under the power cap); forward, so many that their rows of X are
+// about 32 MB (16 at K=4096: 345 us against 351 for 8 and 367 for 4).
+constexpr int GROUP_BACK = 8;
+constexpr uint64_t GROUP_X_BYTES = 32ull << 20;
 constexpr int MAX_SPLIT = 4;
 
 constexpr uint32_t SITE_PRODUCER = 0x00070001u;
@@ -96,6 +100,7 @@ struct Params {
     int tiles_dx, tiles_dw; // tiles of dX and of each of dWg, dWu (0: not computed)
     int tiles;              // in all
     int ratio;              // see nth_tile
+    int group_m;            // forward: row-tiles per group
     void* out0;             // H, or dX
     void* out1;             // G (or null), or dWg
     void* out2;             // U (or null), or dWu
@@ -125,10 +130,11 @@ __device__ __forceinline__ Tile find_tile(int t, const Params& p) {
         if (r.which) t -= p.tiles_dw;
     }
     const int tiles_m = (r.rows + 2 * BM - 1) / (2 * BM), tiles_n = (r.cols + TN - 1) / TN;
-    const int group = GROUP_M * tiles_n;
+    const int group_m = BACK ? GROUP_BACK : p.group_m;
+    const int group = group_m * tiles_n;
     const int g = t / group;
-    const int first_m = g * GROUP_M;
-    const int gm = min(tiles_m - first_m, GROUP_M);
+    const int first_m = g * group_m;
+    const int gm = min(tiles_m - first_m, group_m);
     const int q = t - g * group;
     r.mt = first_m + q % gm;
     r.nt = q / gm;
@@ -399,7 +405,6 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
     } else if (warp >= EPI_WARP0) {
         // ------------------------------------------------------------ epilogue (both CTAs)
         const int group = (warp - EPI_WARP0) / EPI_GROUP;         // tiles group, group + 2, ...
-        const int side = ((warp - EPI_WARP0) % EPI_GROUP) >> 2;   // which half of the columns
         const int row = (warp & 3) * 32 + lane;
         const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + group * BN;
         const uint32_t empty = mapa_shared(smem_u32(&bars->tmem_empty[group]), leader_cta);
@@ -416,7 +421,7 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
                 // this pair's part of the sums, column by column over the drained ring
                 float* part = reinterpret_cast<float*>(smem) + row;
 #pragma unroll 1
-                for (int c = side * (BN / 2); c < (side + 1) * (BN / 2); c += 32) {
+                for (int c = 0; c < BN; c += 32) {
                     uint32_t r[32];
                     __syncwarp();
                     tmem_ld_32x32b_x32(t_row + c, r);
@@ -426,14 +431,14 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
                 }
             } else {
 #pragma unroll 1
-                for (int c = side * (TN / 2); c < (side + 1) * (TN / 2); c += 32) {
+                for (int c = 0; c < TN; c += 32) {
                     uint32_t r0[32], r1[32];
                     __syncwarp();
                     tmem_ld_32x32b_x32(t_row + c, r0);
                     if constexpr (!BACK) tmem_ld_32x32b_x32(t_row + BN / 2 + c, r1);
                     tmem_ld_wait_regs(r0);
                     if constexpr (!BACK) tmem_ld_wait_regs(r1);
-                    if (c + 32 == (side + 1) * (TN / 2)) {
+                    if (c + 32 == TN) {
                         // the warp's last columns are in registers: the region may be overwritten
                         tc_fence_before();
                         __syncwarp();
@@ -462,7 +467,7 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
             const int m_warp = tl.mt * 2 * BM + (int)rank * BM + (warp & 3) * 32;
             const uint32_t base = smem_u32(smem) + (uint32_t)row * 4;
             const int c_end = m_warp < tl.rows ? TN : 0;        // (no rows in this warp: nothing)
-            for (int c = ((int)sub + subs * ((warp - EPI_WARP0) >> 2)) * 32; c < c_end; c += subs * 4 * 32) {
+            for (int c = ((int)sub + subs * ((warp - EPI_WARP0) >> 2)) * 32; c < c_end; c += subs * (2 * EPI_GROUP / 4) * 32) {
                 uint32_t r0[32] = {}, r1[32] = {};               // fp32 zeros
                 for (int k = 0; k < min(subs, tl.nk); ++k) {
                     const uint32_t at = mapa_shared(base + (uint32_t)(c * BM) * 4, 2u * k + rank);
@@ -631,7 +636,8 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
         (rc = make_map(&maps.wu, Wu, N, K, 128)))
         return rc;
     for (int i = 0; i < 4; ++i) maps.rows[i >> 1][i & 1] = maps.cols[i >> 1][i & 1] = maps.x;   // not read
-    const Params p{M, N, K, 1, 0, 0, 0, 0, H, G, U, nullptr};
+    const uint64_t group = GROUP_X_BYTES / ((uint64_t)2 * BM * (uint64_t)K * 2);
+    const Params p{M, N, K, 1, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
     const int64_t units = (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN / 2);
     return act == QG_ACT_SILU ? launch<T, false, QG_ACT_SILU>(maps, p, units, ceil_div(K, BK), stream)
                               : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
@@ -682,7 +688,7 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     const int nk_dx = 2 * parts * ceil_div(N, BK), nk_dw = parts * ceil_div(M, BK);
     const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
     const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
-    const Params p{M, N, K, parts, 0, 0, 0, (nk_dx + nk_dw / 2) / nk_dw, dX, dWg, dWu, nullptr};
+    const Params p{M, N, K, parts, 0, 0, 0, (nk_dx + nk_dw / 2) / nk_dw, 1, dX, dWg, dWu, nullptr};
     // One launch for the three, unless dX is the long pole: few tiles (few rows of X)
     // of many blocks, which a launch of its own splits, beside many of few blocks.
     // (Decided for all three, whichever are asked for: the same split, the same bits.)
