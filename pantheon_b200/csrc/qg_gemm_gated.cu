@@ -100,6 +100,7 @@ struct Params {
     int tiles_dx, tiles_dw; // tiles of dX and of each of dWg, dWu (0: not computed)
     int tiles;              // in all
     int ratio;              // see nth_tile
+    int whole_from;         // SPLIT: tiles from this one on are not split
     int group_m;            // forward: row-tiles per group
     void* out0;             // H, or dX
     void* out1;             // G (or null), or dWg
@@ -144,10 +145,8 @@ __device__ __forceinline__ Tile find_tile(int t, const Params& p) {
 // The n-th tile of a pair (p.tiles or more: none).  Tiles go round the pairs; where
 // dX leaves some pairs one of its tiles short, those take as many more tiles of
 // dWg and dWu first (`ratio` = blocks of a dX tile per block of a dW tile).
-// A split cluster has the one tile of its number.
-template <bool BACK, bool SPLIT>
+template <bool BACK>
 __device__ __forceinline__ int nth_tile(int n, int pair, int pairs, const Params& p) {
-    if (SPLIT) return n == 0 ? pair : p.tiles;
     const int extra = BACK ? p.tiles_dx % pairs : 0;          // pairs with one dX tile more
     if (extra == 0 || p.tiles_dw == 0) return pair + n * pairs;
     const int mine = p.tiles_dx / pairs + (pair < extra ? 1 : 0);
@@ -159,6 +158,13 @@ __device__ __forceinline__ int nth_tile(int n, int pair, int pairs, const Params
         n -= p.ratio;
     }
     return p.tiles_dx + others * p.ratio + pair + n * pairs;
+}
+
+// The one tile of pair `sub` in cluster `c` of a SPLIT launch: the cluster's own, of
+// which it takes a part, or from p.whole_from on one for each pair (p.tiles or
+// more: none).
+__device__ __forceinline__ int cluster_tile(int c, int sub, int subs, const Params& p) {
+    return c < p.whole_from ? c : p.whole_from + (c - p.whole_from) * subs + sub;
 }
 
 // Where pair `sub` of `subs` begins in a tile of nk blocks.  A tile of fewer
@@ -288,8 +294,13 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
     const uint32_t leader_cta = crank & ~1u;
     const bool leader = rank == 0;
     const int subs = SPLIT ? (int)(cluster_nctas() >> 1) : 1;
-    const int pair = SPLIT ? (int)blockIdx.x / (2 * subs) : (int)blockIdx.x >> 1;
-    const int pairs = (int)gridDim.x >> 1;                  // (not of use to a split cluster)
+    const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+    const int cluster = (int)blockIdx.x / (2 * subs);       // SPLIT: all that the pairs do is in here
+    const bool parted = SPLIT && cluster < p.whole_from;    // and whether it is a part of a tile
+    auto tile_at = [&](int n) {
+        if constexpr (SPLIT) return n == 0 ? cluster_tile(cluster, (int)sub, subs, p) : p.tiles;
+        else return nth_tile<BACK>(n, pair, pairs, p);
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
@@ -316,9 +327,9 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
         // ------------------------------------------------------------ producer (both CTAs)
         uint32_t stage = 0, phase = 0, armed = 0, armed_phase = 0;
         bool ok = true;
-        for (int n = 0, t; ok && (t = nth_tile<BACK, SPLIT>(n, pair, pairs, p)) < p.tiles; ++n) {
+        for (int n = 0, t; ok && (t = tile_at(n)) < p.tiles; ++n) {
             const Tile tl = find_tile<BACK>(t, p);
-            const int i0 = SPLIT ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = SPLIT ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
+            const int i0 = parted ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = parted ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
             const int m0 = tl.mt * 2 * BM + (int)rank * BM;
             const int nb = (p.N + BK - 1) / BK;
             for (int i = i0; i < i1; ++i) {
@@ -363,9 +374,9 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
         uint32_t stage = 0, phase = 0;
         bool ok = true, issued = false;
         int unit = 0;
-        for (int n = 0, t; ok && (t = nth_tile<BACK, SPLIT>(n, pair, pairs, p)) < p.tiles; ++n, ++unit) {
+        for (int n = 0, t; ok && (t = tile_at(n)) < p.tiles; ++n, ++unit) {
             const Tile tl = find_tile<BACK>(t, p);
-            const int i0 = SPLIT ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = SPLIT ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
+            const int i0 = parted ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = parted ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
             auto blocks = [&](auto a_major) {
                 constexpr bool A_IS_MN = decltype(a_major)::value;
                 const uint64_t a_desc = A_IS_MN ? make_sdesc_mnmajor_sw128(a_addr) : make_sdesc_kmajor_sw128(a_addr);
@@ -410,14 +421,14 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
         const uint32_t empty = mapa_shared(smem_u32(&bars->tmem_empty[group]), leader_cta);
         uint32_t use = 0;
         for (int unit = group;; unit += 2, ++use) {
-            const int t = nth_tile<BACK, SPLIT>(unit, pair, pairs, p);
+            const int t = tile_at(unit);
             if (t >= p.tiles) break;
             const Tile tl = find_tile<BACK>(t, p);
             const int m_warp = tl.mt * 2 * BM + (int)rank * BM + (warp & 3) * 32;
-            if (SPLIT && ((int)sub >= tl.nk || m_warp >= tl.rows)) break;   // no blocks or no rows: no part
+            if (parted && ((int)sub >= tl.nk || m_warp >= tl.rows)) break;   // no blocks or no rows: no part
             if (!warp_wait(&bars->tmem_full[group], use & 1, abort_flag, p.status, SITE_EPI)) break;
             tc_fence_after();
-            if constexpr (SPLIT) {
+            if (parted) {
                 // this pair's part of the sums, column by column over the drained ring
                 float* part = reinterpret_cast<float*>(smem) + row;
 #pragma unroll 1
@@ -461,8 +472,8 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
     }
     if constexpr (SPLIT) {
         // every CTA joins its share of the columns, 32 at a time, from the same CTA of each pair
-        if (warp >= EPI_WARP0) {
-            const Tile tl = find_tile<BACK>(pair, p);
+        if (warp >= EPI_WARP0 && parted) {
+            const Tile tl = find_tile<BACK>(cluster, p);
             const int row = (warp & 3) * 32 + lane;
             const int m_warp = tl.mt * 2 * BM + (int)rank * BM + (warp & 3) * 32;
             const uint32_t base = smem_u32(smem) + (uint32_t)row * 4;
@@ -568,7 +579,11 @@ static int launch_kernel(const Maps& maps, Params p, int subs, const DeviceInfo*
     auto kernel = gated_kernel<T, BACK, ACT, SPLIT>;
     QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
     int pairs = 0;
-    if constexpr (SPLIT) pairs = p.tiles * subs;
+    if constexpr (SPLIT) {
+        // (a backward pass splits all its tiles, or those of dX)
+        p.whole_from = p.whole_from ? p.tiles_dx : p.tiles;
+        pairs = (p.whole_from + ceil_div(p.tiles - p.whole_from, subs)) * subs;
+    }
     else {
         int rc = resident_clusters(kernel, 2, &pairs, info);
         if (rc) return rc;
@@ -637,7 +652,7 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
         return rc;
     for (int i = 0; i < 4; ++i) maps.rows[i >> 1][i & 1] = maps.cols[i >> 1][i & 1] = maps.x;   // not read
     const uint64_t group = GROUP_X_BYTES / ((uint64_t)2 * BM * (uint64_t)K * 2);
-    const Params p{M, N, K, 1, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
+    const Params p{M, N, K, 1, 0, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
     const int64_t units = (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN / 2);
     return act == QG_ACT_SILU ? launch<T, false, QG_ACT_SILU>(maps, p, units, ceil_div(K, BK), stream)
                               : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
@@ -688,17 +703,32 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     const int nk_dx = 2 * parts * ceil_div(N, BK), nk_dw = parts * ceil_div(M, BK);
     const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
     const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
-    const Params p{M, N, K, parts, 0, 0, 0, (nk_dx + nk_dw / 2) / nk_dw, 1, dX, dWg, dWu, nullptr};
-    // One launch for the three, unless dX is the long pole: few tiles (few rows of X)
-    // of many blocks, which a launch of its own splits, beside many of few blocks.
-    // (Decided for all three, whichever are asked for: the same split, the same bits.)
+    const Params p{M, N, K, parts, 0, 0, 0, (nk_dx + nk_dw / 2) / nk_dw, 0, 1, dX, dWg, dWu, nullptr};
+    // One launch for the three: all tiles split, or those of dX, where it is the long
+    // pole (few tiles of many blocks, from few rows of X, beside many of few) and all
+    // fit at once; or none split.  Where dX is the long pole and they do not fit, dX
+    // goes alone, split, and dWg and dWu follow.  (Decided for all three, whichever are
+    // asked for: the same split, the same bits.)
     const int nk = nk_dx > nk_dw ? nk_dx : nk_dw;
-    int all = 1, alone = 1;
+    int all = 1, alone = 1, beside = 1;
     if ((rc = pick_split<T, true, QG_ACT_SILU>(&all, units_dx + units_dw, nk, info)) ||
         (rc = pick_split<T, true, QG_ACT_SILU>(&alone, units_dx, nk_dx, info)))
         return rc;
     if (all == 1 && alone > 1 && nk_dx > 2 * nk_dw) {
+        for (int s = 2; s <= MAX_SPLIT; s *= 2) {
+            int clusters = 0;
+            if ((rc = resident_clusters(gated_kernel<T, true, QG_ACT_SILU, true>, 2 * s, &clusters, info))) return rc;
+            if (units_dx + (units_dw + s - 1) / s <= clusters) beside = s;
+        }
         Params q = p;
+        q.tiles_dx = dX ? 1 : 0;
+        q.tiles_dw = dWg ? 1 : 0;
+        q.whole_from = 1;
+        if (beside > 1) {
+            if ((rc = device_status_ptr(&q.status))) return rc;
+            return launch_kernel<T, true, QG_ACT_SILU, true>(maps, q, beside, info, stream);
+        }
+        q = p;
         q.tiles_dx = 1;
         if (dX && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_dx, nk_dx, stream))) return rc;
         q = p;
