@@ -99,6 +99,8 @@ struct Params {
     int parts;              // terms of dG and dU (1 or 2)
     int tiles_dx, tiles_dw; // tiles of dX and of each of dWg, dWu (0: not computed)
     int tiles;              // in all
+    int first;              // of them those with the longer contraction come first: dX's,
+    int dw_first;           // or dWg's and dWu's
     int ratio;              // see nth_tile
     int whole_from;         // SPLIT: tiles from this one on are not split
     int group_m;            // forward: row-tiles per group
@@ -123,12 +125,15 @@ __device__ __forceinline__ Tile find_tile(int t, const Params& p) {
     Tile r;
     if constexpr (!BACK) {
         r.kind = FWD; r.which = 0; r.rows = p.M; r.cols = p.N; r.nk = (p.K + BK - 1) / BK;
-    } else if (t < p.tiles_dx) {
-        r.kind = DX; r.which = 0; r.rows = p.M; r.cols = p.K; r.nk = 2 * p.parts * ((p.N + BK - 1) / BK);
     } else {
-        t -= p.tiles_dx;
-        r.kind = DW; r.which = t >= p.tiles_dw; r.rows = p.N; r.cols = p.K; r.nk = p.parts * ((p.M + BK - 1) / BK);
-        if (r.which) t -= p.tiles_dw;
+        const bool head = t < p.first;
+        if (!head) t -= p.first;
+        if (head != (p.dw_first != 0)) {
+            r.kind = DX; r.which = 0; r.rows = p.M; r.cols = p.K; r.nk = 2 * p.parts * ((p.N + BK - 1) / BK);
+        } else {
+            r.kind = DW; r.which = t >= p.tiles_dw; r.rows = p.N; r.cols = p.K; r.nk = p.parts * ((p.M + BK - 1) / BK);
+            if (r.which) t -= p.tiles_dw;
+        }
     }
     const int tiles_m = (r.rows + 2 * BM - 1) / (2 * BM), tiles_n = (r.cols + TN - 1) / TN;
     const int group_m = BACK ? GROUP_BACK : p.group_m;
@@ -143,21 +148,21 @@ __device__ __forceinline__ Tile find_tile(int t, const Params& p) {
 }
 
 // The n-th tile of a pair (p.tiles or more: none).  Tiles go round the pairs; where
-// dX leaves some pairs one of its tiles short, those take as many more tiles of
-// dWg and dWu first (`ratio` = blocks of a dX tile per block of a dW tile).
+// the long ones leave some pairs one short, those take as many more of the short
+// ones first (`ratio` = blocks of a long tile per block of a short one).
 template <bool BACK>
 __device__ __forceinline__ int nth_tile(int n, int pair, int pairs, const Params& p) {
-    const int extra = BACK ? p.tiles_dx % pairs : 0;          // pairs with one dX tile more
-    if (extra == 0 || p.tiles_dw == 0) return pair + n * pairs;
-    const int mine = p.tiles_dx / pairs + (pair < extra ? 1 : 0);
+    const int extra = BACK ? p.first % pairs : 0;             // pairs with one long tile more
+    if (extra == 0 || p.first == p.tiles) return pair + n * pairs;
+    const int mine = p.first / pairs + (pair < extra ? 1 : 0);
     if (n < mine) return pair + n * pairs;
     n -= mine;
     const int others = pairs - extra;
     if (pair >= extra) {
-        if (n < p.ratio) return p.tiles_dx + (pair - extra) + n * others;
+        if (n < p.ratio) return p.first + (pair - extra) + n * others;
         n -= p.ratio;
     }
-    return p.tiles_dx + others * p.ratio + pair + n * pairs;
+    return p.first + others * p.ratio + pair + n * pairs;
 }
 
 // The one tile of pair `sub` in cluster `c` of a SPLIT launch: the cluster's own, of
@@ -575,13 +580,14 @@ static int launch_kernel(const Maps& maps, Params p, int subs, const DeviceInfo*
         if (p.tiles_dx) p.tiles_dx = ceil_div(p.M, 2 * BM) * ceil_div(p.K, TN);
         if (p.tiles_dw) p.tiles_dw = ceil_div(p.N, 2 * BM) * ceil_div(p.K, TN);
         p.tiles = p.tiles_dx + 2 * p.tiles_dw;
+        p.first = p.dw_first ? 2 * p.tiles_dw : p.tiles_dx;
     }
     auto kernel = gated_kernel<T, BACK, ACT, SPLIT>;
     QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
     int pairs = 0;
     if constexpr (SPLIT) {
-        // (a backward pass splits all its tiles, or those of dX)
-        p.whole_from = p.whole_from ? p.tiles_dx : p.tiles;
+        // (a backward pass splits all its tiles, or the long ones)
+        p.whole_from = p.whole_from ? p.first : p.tiles;
         pairs = (p.whole_from + ceil_div(p.tiles - p.whole_from, subs)) * subs;
     }
     else {
@@ -652,7 +658,7 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
         return rc;
     for (int i = 0; i < 4; ++i) maps.rows[i >> 1][i & 1] = maps.cols[i >> 1][i & 1] = maps.x;   // not read
     const uint64_t group = GROUP_X_BYTES / ((uint64_t)2 * BM * (uint64_t)K * 2);
-    const Params p{M, N, K, 1, 0, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
+    const Params p{M, N, K, 1, 0, 0, 0, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
     const int64_t units = (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN / 2);
     return act == QG_ACT_SILU ? launch<T, false, QG_ACT_SILU>(maps, p, units, ceil_div(K, BK), stream)
                               : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
@@ -703,43 +709,40 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     const int nk_dx = 2 * parts * ceil_div(N, BK), nk_dw = parts * ceil_div(M, BK);
     const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
     const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
-    const Params p{M, N, K, parts, 0, 0, 0, (nk_dx + nk_dw / 2) / nk_dw, 0, 1, dX, dWg, dWu, nullptr};
-    // One launch for the three: all tiles split, or those of dX, where it is the long
-    // pole (few tiles of many blocks, from few rows of X, beside many of few) and all
-    // fit at once; or none split.  Where dX is the long pole and they do not fit, dX
-    // goes alone, split, and dWg and dWu follow.  (Decided for all three, whichever are
-    // asked for: the same split, the same bits.)
-    const int nk = nk_dx > nk_dw ? nk_dx : nk_dw;
+    // One launch for the three: all tiles split; or the long ones, where they are few of
+    // many blocks beside many of few (dX with few rows of X, dWg and dWu with many) and
+    // all fit at once; or none split.  Where the long ones should be split and do not
+    // fit beside the others, they go alone and the others follow.  (Decided for all
+    // three, whichever are asked for: the same split, the same bits.)
+    const bool dw_first = nk_dw > nk_dx;
+    const int nk = dw_first ? nk_dw : nk_dx, nk_short = dw_first ? nk_dx : nk_dw;
+    const int64_t units = dw_first ? units_dw : units_dx, units_short = dw_first ? units_dx : units_dw;
+    const Params p{M, N, K, parts, dX ? 1 : 0, dWg ? 1 : 0, 0, 0, dw_first, (nk + nk_short / 2) / nk_short, 0, 1, dX, dWg,
+                   dWu, nullptr};
     int all = 1, alone = 1, beside = 1;
-    if ((rc = pick_split<T, true, QG_ACT_SILU>(&all, units_dx + units_dw, nk, info)) ||
-        (rc = pick_split<T, true, QG_ACT_SILU>(&alone, units_dx, nk_dx, info)))
+    if ((rc = pick_split<T, true, QG_ACT_SILU>(&all, units + units_short, nk, info)) ||
+        (rc = pick_split<T, true, QG_ACT_SILU>(&alone, units, nk, info)))
         return rc;
-    if (all == 1 && alone > 1 && nk_dx > 2 * nk_dw) {
+    if (all == 1 && alone > 1 && nk > 2 * nk_short) {
         for (int s = 2; s <= MAX_SPLIT; s *= 2) {
             int clusters = 0;
             if ((rc = resident_clusters(gated_kernel<T, true, QG_ACT_SILU, true>, 2 * s, &clusters, info))) return rc;
-            if (units_dx + (units_dw + s - 1) / s <= clusters) beside = s;
+            if (units + (units_short + s - 1) / s <= clusters) beside = s;
         }
         Params q = p;
-        q.tiles_dx = dX ? 1 : 0;
-        q.tiles_dw = dWg ? 1 : 0;
-        q.whole_from = 1;
         if (beside > 1) {
+            q.whole_from = 1;
             if ((rc = device_status_ptr(&q.status))) return rc;
             return launch_kernel<T, true, QG_ACT_SILU, true>(maps, q, beside, info, stream);
         }
+        (dw_first ? q.tiles_dx : q.tiles_dw) = 0;
+        if ((dw_first ? dWg : dX) && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units, nk, stream))) return rc;
         q = p;
-        q.tiles_dx = 1;
-        if (dX && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_dx, nk_dx, stream))) return rc;
-        q = p;
-        q.tiles_dw = 1;
-        if (dWg && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_dw, nk_dw, stream))) return rc;
+        (dw_first ? q.tiles_dw : q.tiles_dx) = 0;
+        if ((dw_first ? dX : dWg) && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_short, nk_short, stream))) return rc;
         return QG_OK;
     }
-    Params q = p;
-    q.tiles_dx = dX ? 1 : 0;
-    q.tiles_dw = dWg ? 1 : 0;
-    return launch<T, true, QG_ACT_SILU>(maps, q, units_dx + units_dw, nk, stream);
+    return launch<T, true, QG_ACT_SILU>(maps, p, units + units_short, nk, stream);
 }
 
 } // namespace ffn

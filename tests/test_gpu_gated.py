@@ -100,11 +100,13 @@ def test_backward_matches_the_formula(cuda_device, shape, act, kind):
 
 # several tiles per CTA pair (forward 96 tiles; backward 165 tiles of two lengths), dX split alone
 # beside whole dWg and dWu, two-term gradients at their limit of 256 rows, all three split with tiles
-# of dWg and dWu the longer ones, and dX split in two or four with whole dWg and dWu in one launch
+# of dWg and dWu the longer ones, dX split in two or four with whole dWg and dWu in one launch, and
+# dWg and dWu split beside a whole dX or before it
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("shape", [(700, 4000, 136), (1100, 1032, 2600), (100, 5000, 256), (256, 512, 776),
                                    (257, 512, 776), (2000, 64, 256), (1500, 136, 72), (515, 1368, 520),
-                                   (200, 1368, 520)],
+                                   (200, 1368, 520), (4096, 512, 264), (2600, 1032, 776), (20000, 256, 512),
+                                   (100, 12000, 512)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_larger_shapes(cuda_device, shape, kind):
     x, wg, wu = _inputs(shape, kind, cuda_device)
