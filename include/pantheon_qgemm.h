@@ -354,12 +354,13 @@ QG_API int  qg_gemm_gated_f16(const void* X, const void* Wg, const void* Wu, voi
                               int M, int N, int K, void* stream);
 
 /* The backward pass, from dH [M,N] and what the forward pass read and kept:
- *   dG = dH * U * act'(G), dU = dH * act(G)        (rounded to the type)
+ *   dG = dH * U * act'(G), dU = dH * act(G)        (rounded to the type where
+ *                                                   M N > 65536)
  *   dX = dG Wg + dU Wu [M,K],  dWg = dG^T X, dWu = dU^T X [N,K]
  * fp32 accumulate, results of the operands' type (written, not added to).  dX, or
  * dWg and dWu together, may be null: not computed.  `workspace`
  * (qg_gemm_gated_backward_workspace_bytes, 16-byte aligned, any contents) holds
- * dG and dU (up to 256 rows with what their rounding left out); calls that share one must not overlap on the GPU.
+ * dG and dU (with what their rounding left out, where M N <= 65536); calls that share one must not overlap on the GPU.
  * No counterpart in the reference. */
 QG_API int  qg_gemm_gated_backward_workspace_bytes(int M, int N, uint64_t* bytes);
 QG_API int  qg_gemm_gated_bf16_backward(const void* dH, const void* X, const void* Wg, const void* Wu, const void* G,

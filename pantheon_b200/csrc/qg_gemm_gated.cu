@@ -27,10 +27,11 @@
 // and every CTA joins a share of the columns over distributed shared memory, in
 // rank order (the same bits on every run, no workspace).
 // dG and dU are operands of the tensor cores, so rounded to the type: an error of
-// half a step in each, of the size of the result's own rounding.  Up to 256 rows
-// of X, where few values meet in a sum and the time is that of the weights'
-// bytes, they go as two terms (value and remainder, `parts` = 2): the weights'
-// block is read again from L2 and the rounding is gone.
+// half a step in each, of the size of the result's own rounding.  Where they hold
+// few values (M N <= 65536), a handful of which can carry a sum, they go as two
+// terms (value and remainder; a stage then holds both beside one block of B) and
+// that rounding is gone; such calls last as long as their launches.  With more
+// values the second term's products would count (16x8192x4096: dX 80 us for 45).
 // G and U as kept are rounded likewise; H comes from the unrounded sums.
 // All barrier waits are bounded (qg_ptx.cuh).
 #include "qg_common.cuh"
@@ -59,9 +60,11 @@ constexpr int BK = 64;                      // contraction elements per stage: 1
 constexpr int UMMA_K = 16;
 constexpr int OP_BYTES = 128 * BK * 2;      // 16 KB: 128 rows of an operand
 constexpr int MN_BLOCK = 64 * BK * 2;       // 8 KB: 64 columns x 64 contraction rows of an MN-major operand
-constexpr int STAGES = 6;
-constexpr int STAGE_BYTES = 2 * OP_BYTES;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+// Stages of the ring: A and B, or A in two terms and B; 192 KB either way.
+__host__ __device__ constexpr int stages(int parts) { return parts == 2 ? 4 : 6; }
+constexpr int RING_BYTES = 192 * 1024;
+static_assert(stages(1) * 2 * OP_BYTES == RING_BYTES && stages(2) * 3 * OP_BYTES == RING_BYTES, "ring");
+constexpr int SMEM_BYTES = RING_BYTES + 1024 + 256;
 constexpr int EPI_WARP0 = 4;
 constexpr int EPI_GROUP = 4;                // epilogue warps of a region, one per TMEM lane quarter (two: 368 us against 350)
 constexpr int THREADS = (EPI_WARP0 + 2 * EPI_GROUP) * 32;
@@ -78,8 +81,8 @@ constexpr uint32_t SITE_MMA_TMEM = 0x00070003u;
 constexpr uint32_t SITE_EPI = 0x00070004u;
 
 struct Barriers {
-    uint64_t full[STAGES];
-    uint64_t empty[STAGES];
+    uint64_t full[6];
+    uint64_t empty[6];
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint64_t drain;
@@ -96,7 +99,6 @@ struct Maps {
 
 struct Params {
     int M, N, K;
-    int parts;              // terms of dG and dU (1 or 2)
     int tiles_dx, tiles_dw; // tiles of dX and of each of dWg, dWu (0: not computed)
     int tiles;              // in all
     int first;              // of them those with the longer contraction come first: dX's,
@@ -129,9 +131,9 @@ __device__ __forceinline__ Tile find_tile(int t, const Params& p) {
         const bool head = t < p.first;
         if (!head) t -= p.first;
         if (head != (p.dw_first != 0)) {
-            r.kind = DX; r.which = 0; r.rows = p.M; r.cols = p.K; r.nk = 2 * p.parts * ((p.N + BK - 1) / BK);
+            r.kind = DX; r.which = 0; r.rows = p.M; r.cols = p.K; r.nk = 2 * ((p.N + BK - 1) / BK);
         } else {
-            r.kind = DW; r.which = t >= p.tiles_dw; r.rows = p.N; r.cols = p.K; r.nk = p.parts * ((p.M + BK - 1) / BK);
+            r.kind = DW; r.which = t >= p.tiles_dw; r.rows = p.N; r.cols = p.K; r.nk = (p.M + BK - 1) / BK;
             if (r.which) t -= p.tiles_dw;
         }
     }
@@ -278,10 +280,11 @@ __device__ __forceinline__ void finish32(const Params& p, const Tile& tl, int ro
     }
 }
 
-template <typename T, bool BACK, int ACT, bool SPLIT>
+template <typename T, bool BACK, int ACT, bool SPLIT, int PARTS>   // PARTS: terms of dG and dU
 __global__ void __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ Maps maps, const Params p) {
     constexpr int TN = BACK ? BN : BN / 2;                  // output columns of a tile
+    constexpr int STAGES = stages(PARTS), A_BYTES = PARTS * OP_BYTES;
     constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t IDESC = make_idesc(1, FMT, FMT, 2 * BM, BN);
     constexpr uint32_t A_MN = 1u << 15, B_MN = 1u << 16;
@@ -289,8 +292,8 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
     uint8_t* sA = smem;
-    uint8_t* sB = smem + STAGES * OP_BYTES;
-    Barriers* bars = reinterpret_cast<Barriers*>(smem + STAGES * STAGE_BYTES);
+    uint8_t* sB = smem + STAGES * A_BYTES;
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);   // uniform, and known to be
     const int lane = threadIdx.x & 31;
@@ -339,25 +342,27 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
             const int nb = (p.N + BK - 1) / BK;
             for (int i = i0; i < i1; ++i) {
                 if (!mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER)) { ok = false; break; }
-                if (leader) mbar_arrive_expect_tx(&bars->full[stage], 2 * STAGE_BYTES);
+                if (leader) mbar_arrive_expect_tx(&bars->full[stage], 2 * (A_BYTES + OP_BYTES));
                 const uint32_t full = mapa_shared(smem_u32(&bars->full[stage]), leader_cta);
-                uint8_t* da = sA + stage * OP_BYTES;
+                uint8_t* da = sA + stage * A_BYTES;
                 uint8_t* db = sB + stage * OP_BYTES;
                 if constexpr (!BACK) {
                     load_operand<false>(da, &maps.x, full, m0, i * BK);
                     load_operand<false>(db, leader ? &maps.wg : &maps.wu, full, tl.nt * 128, i * BK);
                 } else {
                     int j = i;
-                    const int part = p.parts == 2 ? (j & 1) : 0;
-                    if (p.parts == 2) j >>= 1;
                     const CUtensorMap* b = &maps.x;
                     if (tl.kind == DX) {
                         const int seg = j >= nb;
                         if (seg) j -= nb;
                         b = seg ? &maps.wu : &maps.wg;
-                        load_operand<false>(da, &maps.rows[seg][part], full, m0, j * BK);
+#pragma unroll
+                        for (int q = 0; q < PARTS; ++q)
+                            load_operand<false>(da + q * OP_BYTES, &maps.rows[seg][q], full, m0, j * BK);
                     } else {
-                        load_operand<true>(da, &maps.cols[tl.which][part], full, m0, j * BK);
+#pragma unroll
+                        for (int q = 0; q < PARTS; ++q)
+                            load_operand<true>(da + q * OP_BYTES, &maps.cols[tl.which][q], full, m0, j * BK);
                     }
                     load_operand<true>(db, b, full, tl.nt * BN + (int)rank * 128, j * BK);
                 }
@@ -397,11 +402,13 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
                         return false;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t ad = a_desc + stage * (OP_BYTES >> 4), bd = b_desc + stage * (OP_BYTES >> 4);
+                        const uint64_t ad = a_desc + stage * (A_BYTES >> 4), bd = b_desc + stage * (OP_BYTES >> 4);
 #pragma unroll
-                        for (int k = 0; k < BK / UMMA_K; ++k)
-                            umma_f16_pair(tmem_base + region * BN, ad + k * A_STEP, bd + k * B_STEP, ID,
-                                          i != i0 || k != 0 ? 1u : 0u);
+                        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                            for (int k = 0; k < BK / UMMA_K; ++k)
+                                umma_f16_pair(tmem_base + region * BN, ad + q * (OP_BYTES >> 4) + k * A_STEP, bd + k * B_STEP,
+                                              ID, i != i0 || (q | k) != 0 ? 1u : 0u);
                         umma_commit_both(&bars->empty[stage], sub);
                         if (i + 1 == i1) umma_commit_both(&bars->tmem_full[region], sub);
                     }
@@ -572,7 +579,7 @@ static int resident_clusters(void (*kernel)(Maps, Params), int ctas, int* out, c
     return QG_OK;
 }
 
-template <typename T, bool BACK, int ACT, bool SPLIT>
+template <typename T, bool BACK, int ACT, bool SPLIT, int PARTS>
 static int launch_kernel(const Maps& maps, Params p, int subs, const DeviceInfo* info, cudaStream_t stream) {
     constexpr int TN = BACK ? BN : BN / 2;
     if constexpr (!BACK) p.tiles = ceil_div(p.M, 2 * BM) * ceil_div(p.N, TN);
@@ -582,7 +589,7 @@ static int launch_kernel(const Maps& maps, Params p, int subs, const DeviceInfo*
         p.tiles = p.tiles_dx + 2 * p.tiles_dw;
         p.first = p.dw_first ? 2 * p.tiles_dw : p.tiles_dx;
     }
-    auto kernel = gated_kernel<T, BACK, ACT, SPLIT>;
+    auto kernel = gated_kernel<T, BACK, ACT, SPLIT, PARTS>;
     QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
     int pairs = 0;
     if constexpr (SPLIT) {
@@ -610,14 +617,14 @@ static int pick_split(int* out, int64_t units, int nk, const DeviceInfo* info) {
     *out = 1;
     for (int s = 2; s <= MAX_SPLIT && nk >= SPLIT_MIN_BLOCKS; s *= 2) {
         int clusters = 0;
-        const int rc = resident_clusters(gated_kernel<T, BACK, ACT, true>, 2 * s, &clusters, info);
+        const int rc = resident_clusters(gated_kernel<T, BACK, ACT, true, 1>, 2 * s, &clusters, info);
         if (rc) return rc;
         if (units <= clusters) *out = s;
     }
     return QG_OK;
 }
 
-template <typename T, bool BACK, int ACT>
+template <typename T, bool BACK, int ACT, int PARTS = 1>
 static int launch(const Maps& maps, Params p, int64_t units, int nk, cudaStream_t stream) {
     DeviceInfo* info = nullptr;
     int rc = current_device_info(&info);
@@ -625,8 +632,8 @@ static int launch(const Maps& maps, Params p, int64_t units, int nk, cudaStream_
     if ((rc = device_status_ptr(&p.status))) return rc;
     int subs = 1;
     if ((rc = pick_split<T, BACK, ACT>(&subs, units, nk, info))) return rc;
-    return subs > 1 ? launch_kernel<T, BACK, ACT, true>(maps, p, subs, info, stream)
-                    : launch_kernel<T, BACK, ACT, false>(maps, p, 1, info, stream);
+    return subs > 1 ? launch_kernel<T, BACK, ACT, true, PARTS>(maps, p, subs, info, stream)
+                    : launch_kernel<T, BACK, ACT, false, PARTS>(maps, p, 1, info, stream);
 }
 
 static int check_shape(const char* name, int M, int N, int K) {
@@ -640,7 +647,7 @@ static int check_shape(const char* name, int M, int N, int K) {
 }
 
 // Terms of dG and dU (see the head of this file).
-static int grad_parts(int M) { return M <= 2 * BM ? 2 : 1; }
+static int grad_parts(int M, int N) { return (int64_t)M * N <= 65536 ? 2 : 1; }
 
 template <typename T>
 static int forward(const char* name, const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, int act,
@@ -658,10 +665,54 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
         return rc;
     for (int i = 0; i < 4; ++i) maps.rows[i >> 1][i & 1] = maps.cols[i >> 1][i & 1] = maps.x;   // not read
     const uint64_t group = GROUP_X_BYTES / ((uint64_t)2 * BM * (uint64_t)K * 2);
-    const Params p{M, N, K, 1, 0, 0, 0, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
+    const Params p{M, N, K, 0, 0, 0, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
     const int64_t units = (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN / 2);
     return act == QG_ACT_SILU ? launch<T, false, QG_ACT_SILU>(maps, p, units, ceil_div(K, BK), stream)
                               : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
+}
+
+// The three products of the backward pass.
+template <typename T, int PARTS>
+static int products(const Maps& maps, void* dX, void* dWg, void* dWu, int M, int N, int K, const DeviceInfo* info,
+                    cudaStream_t stream) {
+    int rc;
+    const int nk_dx = 2 * ceil_div(N, BK), nk_dw = ceil_div(M, BK);
+    const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
+    const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
+    // One launch for the three: all tiles split; or the long ones, where they are few of
+    // many blocks beside many of few (dX with few rows of X, dWg and dWu with many) and
+    // all fit at once; or none split.  Where the long ones should be split and do not
+    // fit beside the others, they go alone and the others follow.  (Decided for all
+    // three, whichever are asked for: the same split, the same bits.)
+    const bool dw_first = nk_dw > nk_dx;
+    const int nk = dw_first ? nk_dw : nk_dx, nk_short = dw_first ? nk_dx : nk_dw;
+    const int64_t units = dw_first ? units_dw : units_dx, units_short = dw_first ? units_dx : units_dw;
+    const Params p{M, N, K, dX ? 1 : 0, dWg ? 1 : 0, 0, 0, dw_first, (nk + nk_short / 2) / nk_short, 0, 1, dX, dWg,
+                   dWu, nullptr};
+    int all = 1, alone = 1, beside = 1;
+    if ((rc = pick_split<T, true, QG_ACT_SILU>(&all, units + units_short, nk, info)) ||
+        (rc = pick_split<T, true, QG_ACT_SILU>(&alone, units, nk, info)))
+        return rc;
+    if (all == 1 && alone > 1 && nk > 2 * nk_short) {
+        for (int s = 2; s <= MAX_SPLIT; s *= 2) {
+            int clusters = 0;
+            if ((rc = resident_clusters(gated_kernel<T, true, QG_ACT_SILU, true, 1>, 2 * s, &clusters, info))) return rc;
+            if (units + (units_short + s - 1) / s <= clusters) beside = s;
+        }
+        Params q = p;
+        if (beside > 1) {
+            q.whole_from = 1;
+            if ((rc = device_status_ptr(&q.status))) return rc;
+            return launch_kernel<T, true, QG_ACT_SILU, true, PARTS>(maps, q, beside, info, stream);
+        }
+        (dw_first ? q.tiles_dx : q.tiles_dw) = 0;
+        if ((dw_first ? dWg : dX) && (rc = launch<T, true, QG_ACT_SILU, PARTS>(maps, q, units, nk, stream))) return rc;
+        q = p;
+        (dw_first ? q.tiles_dw : q.tiles_dx) = 0;
+        if ((dw_first ? dX : dWg) && (rc = launch<T, true, QG_ACT_SILU, PARTS>(maps, q, units_short, nk_short, stream))) return rc;
+        return QG_OK;
+    }
+    return launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units + units_short, nk, stream);
 }
 
 template <typename T>
@@ -674,7 +725,7 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     QG_CHECK_ARG(act == QG_ACT_SILU || act == QG_ACT_GELU_TANH, "%s: unknown activation %d", name, act);
     int rc = check_shape(name, M, N, K);
     if (rc) return rc;
-    const int parts = grad_parts(M);
+    const int parts = grad_parts(M, N);
     const uint64_t one = (uint64_t)M * (uint64_t)N * 2;           // a multiple of 16
     QG_CHECK_ARG(workspace && workspace_bytes >= 2 * parts * one, "%s: workspace of %llu bytes, %llu needed", name,
                  (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)(2 * parts * one));
@@ -706,43 +757,8 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     }
     if ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)) || (rc = make_map(&maps.x, X, M, K, BK)))
         return rc;
-    const int nk_dx = 2 * parts * ceil_div(N, BK), nk_dw = parts * ceil_div(M, BK);
-    const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
-    const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
-    // One launch for the three: all tiles split; or the long ones, where they are few of
-    // many blocks beside many of few (dX with few rows of X, dWg and dWu with many) and
-    // all fit at once; or none split.  Where the long ones should be split and do not
-    // fit beside the others, they go alone and the others follow.  (Decided for all
-    // three, whichever are asked for: the same split, the same bits.)
-    const bool dw_first = nk_dw > nk_dx;
-    const int nk = dw_first ? nk_dw : nk_dx, nk_short = dw_first ? nk_dx : nk_dw;
-    const int64_t units = dw_first ? units_dw : units_dx, units_short = dw_first ? units_dx : units_dw;
-    const Params p{M, N, K, parts, dX ? 1 : 0, dWg ? 1 : 0, 0, 0, dw_first, (nk + nk_short / 2) / nk_short, 0, 1, dX, dWg,
-                   dWu, nullptr};
-    int all = 1, alone = 1, beside = 1;
-    if ((rc = pick_split<T, true, QG_ACT_SILU>(&all, units + units_short, nk, info)) ||
-        (rc = pick_split<T, true, QG_ACT_SILU>(&alone, units, nk, info)))
-        return rc;
-    if (all == 1 && alone > 1 && nk > 2 * nk_short) {
-        for (int s = 2; s <= MAX_SPLIT; s *= 2) {
-            int clusters = 0;
-            if ((rc = resident_clusters(gated_kernel<T, true, QG_ACT_SILU, true>, 2 * s, &clusters, info))) return rc;
-            if (units + (units_short + s - 1) / s <= clusters) beside = s;
-        }
-        Params q = p;
-        if (beside > 1) {
-            q.whole_from = 1;
-            if ((rc = device_status_ptr(&q.status))) return rc;
-            return launch_kernel<T, true, QG_ACT_SILU, true>(maps, q, beside, info, stream);
-        }
-        (dw_first ? q.tiles_dx : q.tiles_dw) = 0;
-        if ((dw_first ? dWg : dX) && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units, nk, stream))) return rc;
-        q = p;
-        (dw_first ? q.tiles_dw : q.tiles_dx) = 0;
-        if ((dw_first ? dX : dWg) && (rc = launch<T, true, QG_ACT_SILU>(maps, q, units_short, nk_short, stream))) return rc;
-        return QG_OK;
-    }
-    return launch<T, true, QG_ACT_SILU>(maps, p, units + units_short, nk, stream);
+    return parts == 2 ? products<T, 2>(maps, dX, dWg, dWu, M, N, K, info, stream)
+                      : products<T, 1>(maps, dX, dWg, dWu, M, N, K, info, stream);
 }
 
 } // namespace ffn
@@ -762,7 +778,7 @@ extern "C" int qg_gemm_gated_f16(const void* X, const void* Wg, const void* Wu, 
 
 extern "C" int qg_gemm_gated_backward_workspace_bytes(int M, int N, uint64_t* bytes) {
     QG_CHECK_ARG(bytes && M > 0 && N > 0, "qg_gemm_gated_backward_workspace_bytes: bad argument");
-    *bytes = 4ull * (uint64_t)qg::ffn::grad_parts(M) * (uint64_t)M * (uint64_t)N;
+    *bytes = 4ull * (uint64_t)qg::ffn::grad_parts(M, N) * (uint64_t)M * (uint64_t)N;
     return QG_OK;
 }
 

@@ -380,7 +380,7 @@ def gemm_gated_bf16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor
                              U: torch.Tensor, act: int = QG_ACT_SILU, need_dx: bool = True, need_dw: bool = True,
                              workspace: torch.Tensor | None = None):
     """Gradients (dX, dWg, dWu) of gemm_gated_bf16 from dH [M,N] and the G, U it kept; a gradient
-    that is not needed is None.  Above 256 rows dG and dU are rounded to bf16 on the way.  `workspace` (uint8,
+    that is not needed is None.  Where M N > 65536, dG and dU are rounded to bf16 on the way.  `workspace` (uint8,
     gemm_gated_backward_workspace_bytes) is allocated when not given."""
     return _gemm_gated_backward("qg_gemm_gated_bf16_backward", torch.bfloat16, dH, X, Wg, Wu, G, U, act, need_dx,
                                 need_dw, workspace)

@@ -99,7 +99,7 @@ def test_backward_matches_the_formula(cuda_device, shape, act, kind):
 
 
 # several tiles per CTA pair (forward 96 tiles; backward 165 tiles of two lengths), dX split alone
-# beside whole dWg and dWu, two-term gradients at their limit of 256 rows, all three split with tiles
+# beside whole dWg and dWu, gradients in two terms and in one, all three split with tiles
 # of dWg and dWu the longer ones, dX split in two or four with whole dWg and dWu in one launch, and
 # dWg and dWu split beside a whole dX or before it
 @pytest.mark.parametrize("kind", list(TYPES))
@@ -123,8 +123,8 @@ def test_larger_shapes(cuda_device, shape, kind):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-def test_few_rows_carry_no_intermediate_rounding(cuda_device, kind):
-    """Up to 256 rows dG and dU go as value and remainder: what is left of their rounding is a
+def test_few_values_carry_no_intermediate_rounding(cuda_device, kind):
+    """Up to 65536 values dG and dU go as value and remainder: what is left of their rounding is a
     half step of the remainder, so the results are within their own rounding and the fp32 bounds."""
     M, N, K = 48, 264, 136
     x, wg, wu = _inputs((M, N, K), kind, cuda_device)
