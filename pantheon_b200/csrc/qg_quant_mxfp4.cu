@@ -22,6 +22,7 @@ namespace mx {
 
 constexpr int SEG = 256;        // columns of a warp (dequantisation)
 constexpr int ROWS = 4;         // rows of a warp
+constexpr int ROWS_OFF = 2;     // rows of a warp off 16-byte boundaries (half as many again words per row)
 constexpr int THREADS = 256;
 
 // A lane's 32 bytes of a row.
@@ -31,41 +32,73 @@ struct Raw {
     uint32_t w[8];
 };
 
-// `n` of the values exist, the others are zero.  VEC: rows start on 16 bytes.
+// The aligned 16-byte words around them: two, or three where the row is off a
+// 16-byte boundary.
+template <bool VEC>
+struct Words {
+    uint32_t w[VEC ? 8 : 12];
+};
+
+// Loads a lane's words; `n` of its values exist.  Off the boundary the words reach
+// up to 14 bytes to either side, which is memory of the same tensor as long as
+// they lie in [begin, end), its first and last byte; otherwise (its corners, and
+// rows that end within the lane) the values are loaded one by one, in place.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load(const T* src, int n, Raw<T>& v) {
+__device__ __forceinline__ void load(const T* src, int n, uintptr_t begin, uintptr_t end, Words<VEC>& v) {
     constexpr int N = Raw<T>::N;
-    if (VEC && n == N) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src), base = at & ~(uintptr_t)15;
+    const bool whole = n == N && (VEC || (base >= begin && base + 48 <= end));
+    if (whole) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        for (int i = 0; i < (VEC ? 2 : 3); ++i) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(base) + i);
             v.w[4 * i] = q.x; v.w[4 * i + 1] = q.y; v.w[4 * i + 2] = q.z; v.w[4 * i + 3] = q.w;
         }
-    } else if constexpr (sizeof(T) == 4) {
+        return;
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.w[i] = i < n ? __ldg(reinterpret_cast<const uint32_t*>(src) + i) : 0u;
-    } else {
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-        if (n == N && (reinterpret_cast<uintptr_t>(src) & 2) == 0) {
+    for (int i = 0; i < (VEC ? 8 : 12); ++i) v.w[i] = 0;
+    // as aligned words would hold them: value j at byte (at % 16) + j * sizeof(T)
+    const int off = VEC ? 0 : (int)(at & 15);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
-        } else if (n == N) {
-            // off by half a word: the words between, joined with their neighbours
-            uint32_t lo = __ldg(h);
-#pragma unroll
-            for (int i = 0; i < 7; ++i) {
-                const uint32_t next = __ldg(reinterpret_cast<const uint32_t*>(h + 1) + i);
-                v.w[i] = lo | next << 16;
-                lo = next >> 16;
-            }
-            v.w[7] = lo | (uint32_t)__ldg(h + 15) << 16;
+    for (int i = 0; i < (VEC ? 8 : 12); ++i) {
+        if constexpr (sizeof(T) == 4) {
+            const int j = i - off / 4;
+            if (j >= 0 && j < n) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + j);
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v.w[i] = (2 * i < n ? (uint32_t)__ldg(h + 2 * i) : 0u) |
-                         (2 * i + 1 < n ? (uint32_t)__ldg(h + 2 * i + 1) << 16 : 0u);
+            const int j = 2 * i - off / 2;
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+            if (j >= 0 && j < n) v.w[i] = __ldg(h + j);
+            if (j + 1 >= 0 && j + 1 < n) v.w[i] |= (uint32_t)__ldg(h + j + 1) << 16;
         }
     }
+}
+
+// The lane's bytes out of its words (the offset is the same for the whole warp: a
+// lane is 32 bytes).
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw<T> align(const Words<VEC>& v, const T* src) {
+    Raw<T> r;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.w[i] = v.w[i];
+    } else {
+        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15);
+        uint32_t t[10];
+#pragma unroll
+        for (int i = 0; i < 10; ++i) t[i] = (off & 8) ? v.w[i + 2] : v.w[i];
+#pragma unroll
+        for (int i = 0; i < 9; ++i) t[i] = (off & 4) ? t[i + 1] : t[i];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r.w[i] = t[i];
+        } else {
+            const uint32_t shift = (off & 2) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r.w[i] = __funnelshift_r(t[i], t[i + 1], shift);
+        }
+    }
+    return r;
 }
 
 // Bits of the largest magnitude as its own type's integer: magnitudes of one type
@@ -104,24 +137,29 @@ quant_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q, uint
     const int kp = (K + BLOCK - 1) / BLOCK * BLOCK;          // columns that have codes
     const int kchunks = (K + ATOM_K - 1) / ATOM_K;
     const int segs = (kchunks * ATOM_K + 32 * N - 1) / (32 * N);
-    const int row_groups = (M + 127) / 128 * (128 / ROWS);   // the rows that pad the last atom get zero scales
+    constexpr int R = VEC ? ROWS : ROWS_OFF;
+    const int row_groups = (M + 127) / 128 * (128 / R);      // the rows that pad the last atom get zero scales
     const uint64_t units = (uint64_t)segs * (uint64_t)row_groups;
     wait_previous_grid();
     const uint64_t u = (uint64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
     if (u >= units) return;
     const int rg = (int)(u / (uint32_t)segs);
     const int k0 = (int)(u - (uint64_t)rg * (uint32_t)segs) * (32 * N) + lane * N;
-    const int r0 = rg * ROWS;
+    const int r0 = rg * R;
     const int n = min(N, max(0, K - k0));
-    Raw<T> v[ROWS];
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(X);
+    const uintptr_t end = reinterpret_cast<uintptr_t>(X + (int64_t)(M - 1) * ldx + K);
+    Words<VEC> words[R];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) load<T, VEC>(X + (int64_t)(r0 + i) * ldx + k0, r0 + i < M ? n : 0, v[i]);
+    for (int i = 0; i < R; ++i)
+        load<T, VEC>(X + (int64_t)(r0 + i) * ldx + k0, r0 + i < M ? n : 0, begin, end, words[i]);
     uint8_t* q = Q + (size_t)r0 * (kp / 2) + k0 / 2;
-    // the ROWS rows of a unit follow one another in their atom, 16 bytes apart
+    // the rows of a unit follow one another in their atom, 16 bytes apart
     uint8_t* sf = SF + sf_offset(r0, k0 / BLOCK, kchunks);
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        uint32_t m = max_bits(v[i]);
+    for (int i = 0; i < R; ++i) {
+        const Raw<T> v = align<T, VEC>(words[i], X + (int64_t)(r0 + i) * ldx + k0);
+        uint32_t m = max_bits(v);
 #pragma unroll
         for (int o = 1; o < BLOCK / N; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         const uint32_t s = scale_byte(f32_bits<T>(m));
@@ -131,7 +169,7 @@ quant_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q, uint
         for (int g = 0; g < N / 8; ++g) {
             float f[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = value(v[i], 8 * g + j) * inv;
+            for (int j = 0; j < 8; ++j) f[j] = value(v, 8 * g + j) * inv;
             w[g] = s == 255 ? 0u : pack8(f);
         }
         if (r0 + i < M && k0 < kp) {
@@ -221,10 +259,10 @@ static int launch_quant(const void* X, int64_t ldx, void* Q, void* SF, int M, in
     if (rc) return rc;
     const int width = 32 * Raw<T>::N;
     const int segs = ((K + ATOM_K - 1) / ATOM_K * ATOM_K + width - 1) / width;
-    const uint64_t units = (uint64_t)segs * (uint64_t)((M + 127) / 128 * (128 / ROWS));
+    const bool vec = ((uintptr_t)X & 15) == 0 && (ldx * (int64_t)sizeof(T)) % 16 == 0;
+    const uint64_t units = (uint64_t)segs * (uint64_t)((M + 127) / 128 * (128 / (vec ? ROWS : ROWS_OFF)));
     unsigned grid = 0;
     if ((rc = grid_for(units, "qg_quant_mxfp4", &grid))) return rc;
-    const bool vec = ((uintptr_t)X & 15) == 0 && (ldx * (int64_t)sizeof(T)) % 16 == 0;
     const T* x = static_cast<const T*>(X);
     uint8_t* q = static_cast<uint8_t*>(Q);
     uint8_t* sf = static_cast<uint8_t*>(SF);
