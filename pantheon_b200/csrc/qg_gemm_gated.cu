@@ -33,6 +33,10 @@
 // that rounding is gone; such calls last as long as their launches.  With more
 // values the second term's products would count (16x8192x4096: dX 80 us for 45).
 // G and U as kept are rounded likewise; H comes from the unrounded sums.
+// Bound by the tensor cores: measured at 4096x8192x4096 bf16 the forward pass takes
+// 342-349 us (1.58-1.61 PFLOP/s, 0.93-0.94 of the measured rate, tensor pipe 96 %
+// active), the backward pass 740-760 us (47 of them the stream over M x N, the rest at
+// 97 % of the tensor pipe); back to back under the power cap 410 and 893 us.
 // All barrier waits are bounded (qg_ptx.cuh).
 #include "qg_common.cuh"
 #include "qg_formats.cuh"
@@ -56,7 +60,7 @@ enum : int { FWD = 0, DX = 1, DW = 2 };
 
 constexpr int BM = 128;                     // rows of A per CTA
 constexpr int BN = 256;                     // accumulator columns (rows of B per pair)
-constexpr int BK = 64;                      // contraction elements per stage: 128 bytes
+constexpr int BK = 64;                      // contraction elements per block: 128 bytes
 constexpr int UMMA_K = 16;
 constexpr int OP_BYTES = 128 * BK * 2;      // 16 KB: 128 rows of an operand
 constexpr int MN_BLOCK = 64 * BK * 2;       // 8 KB: 64 columns x 64 contraction rows of an MN-major operand

@@ -4,8 +4,14 @@
 //   C[m,n] = out( sum_k (qa[m,k] 2^ea[m,k/32]) (qb[n,k] 2^eb[n,k/32]) )
 //   gated: H[m,n] = out( act(A Wg^T)[m,n] * (A Wu^T)[m,n] )
 //
-// One persistent CTA per SM, 704 threads, 128 x 256 accumulator columns per
-// tile.  The gated form gives columns 0-127 to Wg and 128-255 to Wu (rows
+// Three kernels (use_rows, launch_gemm): few rows (qg_gemm_mxfp4_rows.cu), single
+// CTAs up to 128 rows, CTA pairs above.  The arithmetic bounds the last: 2 M N K at
+// the fp4 rate; measured 4096x8192x8192 94 us (5.8 PFLOP/s, 0.86 of four times the
+// measured bf16 rate), 8192x8192x16384 341-348 us (6.3-6.4 PFLOP/s, 0.93), tensor pipe
+// 81-86 % active; back to back under the power cap 110 us.
+//
+// Single CTAs: one persistent CTA per SM, 704 threads, 128 x 256 accumulator columns
+// per tile.  The gated form gives columns 0-127 to Wg and 128-255 to Wu (rows
 // [128 nt, 128 nt + 128) of each), so one row's gate and up values lie in the
 // same TMEM lane and the epilogue joins them in registers.
 //   warp 0       producer: per 256-element K block, TMA loads of the A (128
@@ -406,16 +412,17 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 //   * a stage is 512 K (two boxes per operand): the MMA thread's waits cost it
 //     about 350 clocks a stage, against 1024 clocks of MMAs here and 512 with
 //     256 K per stage (111 us at 4096x8192x8192);
-//   * scales have rings of their own, in shared memory
-//     (filled ahead of the codes by warp 22, freed by the writers) and in TMEM
-//     (freed by a commit of the MMAs that read it), so neither a load nor the
-//     writers' round trip lies between a freed code stage and its MMAs;
+//   * scales have rings of their own, in shared memory (filled ahead of the codes by
+//     warp 22, freed by the writers) and in TMEM (freed by a commit of the MMAs that
+//     read it), so neither a load nor the writers' round trip lies between a freed
+//     code stage and its MMAs;
 //   * the writers of both CTAs arrive on the even CTA's `sc_ready`, relaxed: what
 //     they hand over is in TMEM, complete after tcgen05.wait::st and ordered by the
 //     tcgen05 fences on both sides, and a cluster-scope release, which waits for
 //     every access of its thread, took 1400 clocks per K block (157 us in all at
 //     4096x8192x8192);
-//   * the MMA thread commits `empty` and `tmem_full` to both CTAs (plain commits).
+//   * the MMA warp commits to the barriers of both CTAs at once; one elected lane of
+//     the converged warp issues (a lone lane 0 cost 20 %: 147 us against 117).
 constexpr int P_KB = 2;                                        // 256-element K blocks per stage
 constexpr int P_STAGES = 3;                                    // code ring
 constexpr int P_BLOCK_BYTES = 128 * BK_BYTES;                  // 16 KB: a K block of either operand of a CTA

