@@ -375,6 +375,11 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
+        // the even CTA's last commits land here before this CTA's shared memory goes away
+        for (int i = 0; i < STAGES && ok; ++i) {
+            ok = mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
         if (!ok && leader) {
             // copies of both CTAs complete on these barriers: let them land
             for (int s = 0; s < STAGES; ++s)

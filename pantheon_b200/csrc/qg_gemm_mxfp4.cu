@@ -345,6 +345,11 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
+        // the last releases land before the CTA's shared memory goes away
+        for (int i = 0; i < STAGES && ok; ++i) {
+            ok = mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
         if (!ok)
             for (int s = 0; s < STAGES; ++s)
                 if (armed & (1u << s)) mbar_wait(&bars->full[s], (armed_phase >> s) & 1u, nullptr, nullptr, 0);
@@ -555,6 +560,11 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 if (++stage == P_STAGES) { stage = 0; phase ^= 1u; }
             }
         }
+        // the even CTA's last commits land here before this CTA's shared memory goes away
+        for (int i = 0; i < P_STAGES && ok; ++i) {
+            ok = mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER);
+            if (++stage == P_STAGES) { stage = 0; phase ^= 1u; }
+        }
         if (!ok && leader) {
             // copies of both CTAs complete on the even CTA's barriers: let them land
             for (int s = 0; s < P_STAGES; ++s)
@@ -639,11 +649,14 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + BN;
         const int64_t blocks = pair < tiles ? (int64_t)((tiles - pair + pairs - 1) / pairs) * ns : 0;
         uint32_t stage = 0, phase = 0, slot = 0, slot_phase = 0;
+        bool ok = true;
         for (int64_t i = 0; i < blocks; ++i) {
             // the scales have landed, and the MMAs that read these TMEM columns are done
             if (!warp_wait(&bars->sf_full[stage], phase, abort_flag, p.status, SITE_SF) ||
-                !warp_wait(&bars->sc_empty[slot], slot_phase ^ 1u, abort_flag, p.status, SITE_SF))
+                !warp_wait(&bars->sc_empty[slot], slot_phase ^ 1u, abort_flag, p.status, SITE_SF)) {
+                ok = false;
                 break;
+            }
             tc_fence_after();
             // lane i takes bytes [16 i, 16 i + 16) of each atom: four columns.  Atoms past K
             // hold what the stage held before; no MMA reads them.
@@ -670,6 +683,10 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 mbar_arrive(&bars->sf_empty[stage]);
             }
             if (++stage == P_SF_STAGES) { stage = 0; phase ^= 1u; }
+            if (++slot == P_SF_SLOTS) { slot = 0; slot_phase ^= 1u; }
+        }
+        for (int i = 0; i < P_SF_SLOTS && ok; ++i) {          // (as the code producer: the last commits)
+            ok = warp_wait(&bars->sc_empty[slot], slot_phase ^ 1u, abort_flag, p.status, SITE_SF);
             if (++slot == P_SF_SLOTS) { slot = 0; slot_phase ^= 1u; }
         }
     } else if (warp >= EPI_WARP0 && warp < EPI_WARP0 + EPI_WARPS) {

@@ -178,6 +178,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUt
             armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
             if (++stage == G::STAGES) { stage = 0; phase ^= 1u; }
         }
+        // the last releases land before the CTA's shared memory goes away
+        for (int i = 0; i < G::STAGES && ok; ++i) {
+            ok = mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, SITE_PRODUCER);
+            if (++stage == G::STAGES) { stage = 0; phase ^= 1u; }
+        }
         if (!ok)
             for (int s = 0; s < G::STAGES; ++s)
                 if (armed & (1u << s)) mbar_wait(&bars->full[s], (armed_phase >> s) & 1u, nullptr, nullptr, 0);
