@@ -203,6 +203,24 @@ def test_large_arguments(cuda_device, kind):
         assert (np.abs(_np(dx)[:, 0] - 8 * slope[:, 0]) <= 8 * 2 * 1.01 * (TYPES[kind][1] * np.abs(slope[:, 0]) + 1e-5)).all()
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """2.8e9 values of G, U and dH: the last rows of H and dX, and dWg and dWu whose sums have few rows of
+    values other than zero, the last ones."""
+    M, N, K = 70000, 40000, 64
+    g = torch.Generator().manual_seed(11)
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device=cuda_device)
+    x[-40:] = torch.randn((40, K), generator=g).to(torch.bfloat16).to(cuda_device)
+    wg, wu = ((torch.randn((N, K), generator=g) / 4).to(torch.bfloat16).to(cuda_device) for _ in range(2))
+    h, gate, up = pb.gemm_gated_bf16(x, wg, wu, keep=True)
+    _check_forward(x[-40:], wg, wu, 0, "bf16", h[-40:], gate[-40:], up[-40:])
+    assert (h[:-40] == 0).all()
+    dh = torch.zeros_like(h)
+    dh[-40:] = torch.randn((40, N), generator=g).to(torch.bfloat16).to(cuda_device)
+    dx, dwg, dwu = pb.gemm_gated_bf16_backward(dh, x, wg, wu, gate, up)
+    assert (dx[:-40] == 0).all()
+    _check_backward(dh[-40:], x[-40:], wg, wu, gate[-40:], up[-40:], 0, "bf16", (dx[-40:], dwg, dwu))
+
+
 def test_captured_and_replayed_beside_an_eager_call(cuda_device):
     x, wg, wu = _inputs((260, 264, 136), "bf16", cuda_device)
     _, g, u = pb.gemm_gated_bf16(x, wg, wu, keep=True)

@@ -334,3 +334,41 @@ print("captured")
     root = Path(__file__).resolve().parent.parent
     done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Tensors of more than 2^31 values and results of more than 2^31 elements: their last rows."""
+    rows, K = 70016, 32768                                    # 2.29e9 values, 1.15 GB of codes
+    x = torch.zeros((rows, K), dtype=torch.bfloat16, device=cuda_device)
+    last = _values(130, K, seed=9, dtype=torch.bfloat16)
+    x[-130:] = last.to(cuda_device)
+    q, sf = pb.quant_mxfp4(x)
+    code, byte = R.quantise(_np(last))
+    np.testing.assert_array_equal(_np(q[-130:]), R.pack(code, byte)[0])
+    full = sf.view(-1, K // 128, 512)                         # atoms [row block][K chunk]
+    r = np.arange(rows - 130, rows)
+    j = np.arange(K // 32)
+    at = torch.from_numpy((r % 32)[:, None] * 16 + (r // 32 % 4)[:, None] * 4 + j % 4).to(cuda_device)
+    got = full[torch.from_numpy(r // 128).to(cuda_device)[:, None], torch.from_numpy(j // 4).to(cuda_device)[None, :], at]
+    np.testing.assert_array_equal(_np(got), byte)
+    back = pb.dequant_mxfp4(q, sf)
+    np.testing.assert_array_equal(_np(back[-130:]), _np(pb.dequant_mxfp4(*pb.quant_mxfp4(last.to(cuda_device)))))
+    assert (back[:-130] == 0).all()
+    del x, back
+    # as the weights of a product with few rows: code offsets past 32 bits of nibbles and of bytes' bits
+    a, av = _operand(2, K, 5, cuda_device)
+    wv = _np(pb.dequant_mxfp4(*pb.quant_mxfp4(last.to(cuda_device)), pb.QG_OUT_F32))
+    y = pb.gemm_mxfp4(*a, q, sf, out_type=pb.QG_OUT_F32)
+    assert (np.abs(_np(y[:, -130:]) - av @ wv.T) <= R.sum_bound(av, wv)).all() and (y[:, :-130] == 0).all()
+    del q, sf, y
+    # a result of 2.8e9 elements
+    M, N = 70000, 40000
+    a, av = _operand(M, 64, 6, cuda_device)
+    b, bv = _operand(N, 64, 7, cuda_device)
+    p, e = av[-65:] @ bv.T, R.sum_bound(av[-65:], bv)
+    y = pb.gemm_mxfp4(*a, *b)
+    assert (np.abs(_np(y[-65:]) - p) <= e + 2.0 ** -8 * (np.abs(p) + e)).all()
+    y = pb.gemm_gated_mxfp4(*a, *b, *b)
+    with np.errstate(over="ignore"):
+        ref, e = R.activation(p, 0) * p, R.gated_bound(p, p, e, e, 0)
+    assert (np.abs(_np(y[-65:]) - ref) <= e + 2.0 ** -8 * (np.abs(ref) + e)).all()
