@@ -47,6 +47,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <atomic>
 #include <type_traits>
 
 namespace qg {
@@ -565,10 +566,10 @@ static int make_map(CUtensorMap* map, const void* base, int rows, int cols, int 
 // GPC, so this can be below sm_count / ctas).  All forms of the kernel have the
 // same block and shared-memory size, so `kernel` stands for all of them.
 static int resident_clusters(void (*kernel)(Maps, Params), int ctas, int* out, const DeviceInfo* info) {
-    static int known[64][2 * MAX_SPLIT + 1] = {};
+    static std::atomic<int> known[64][2 * MAX_SPLIT + 1];     // 0: not asked yet
     int dev = 0;
     QG_CUDA(cudaGetDevice(&dev));
-    int& res = known[dev & 63][ctas];
+    std::atomic<int>& res = known[dev & 63][ctas];
     if (!res) {
         QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
         cudaLaunchConfig_t lc = {};

@@ -40,6 +40,7 @@
 #include "qg_rows.cuh"
 
 #include <cuda_bf16.h>
+#include <atomic>
 
 namespace qg {
 namespace mx {
@@ -709,7 +710,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 // so this can be below half of the SMs).  All variants have the same block and
 // shared-memory size.
 static int resident_pairs(int* out, const DeviceInfo* info) {
-    static int resident[64] = {};
+    static std::atomic<int> resident[64];                      // 0: not asked yet
     int dev = 0;
     QG_CUDA(cudaGetDevice(&dev));
     if (!resident[dev & 63]) {
