@@ -325,7 +325,8 @@ QG_API int  qg_dequant_mxfp4(const void* Q, const void* SF, void* Y, int out_typ
 
 /* C[m,n] = out( sum_k a[m,k] b[n,k] ) of two MXFP4 tensors A [M,K] and B [N,K]:
  * tensor cores (tcgen05.mma kind::mxf4), fp32 accumulate; any M and N,
- * K % 32 == 0; out_type QG_OUT_BF16 or QG_OUT_F32, C row-major [M,N].
+ * K % 32 == 0; out_type QG_OUT_BF16 or QG_OUT_F32, C row-major [M,N], which
+ * must not overlap an operand.
  * No counterpart in the reference. */
 QG_API int  qg_gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, void* C, int out_type,
                           int M, int N, int K, void* stream);
