@@ -77,6 +77,8 @@ int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, v
 int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void* SFG, const void* Wu, const void* SFU,
                      void* H, void* SFH, int out_type, int act, int M, int N, int K, cudaStream_t stream);
 namespace mx {
+// CTAs that the kernel for few rows gives K to, per tile.
+int rows_split(int M, int N, int K, bool is_gated);
 // Either product for few rows of A (qg_gemm_mxfp4_rows.cu); act < 0 is the plain one.  Arguments are checked by the caller.
 int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,
               void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream);

@@ -4,8 +4,8 @@
 //   C[m,n] = out( sum_k (qa[m,k] 2^ea[m,k/32]) (qb[n,k] 2^eb[n,k/32]) )
 //   gated: H[m,n] = out( act(A Wg^T)[m,n] * (A Wu^T)[m,n] )
 //
-// Three kernels (use_rows, launch_gemm): few rows (qg_gemm_mxfp4_rows.cu), single
-// CTAs up to 128 rows, CTA pairs above.  The arithmetic bounds the last: 2 M N K at
+// Three kernels (use_rows, launch_gemm): few rows or few tiles with a long K
+// (qg_gemm_mxfp4_rows.cu), single CTAs for little work, CTA pairs for the rest.  The arithmetic bounds the last: 2 M N K at
 // the fp4 rate; measured 4096x8192x8192 94 us (5.8 PFLOP/s, 0.86 of four times the
 // measured bf16 rate), 8192x8192x16384 341-348 us (6.3-6.4 PFLOP/s, 0.93), tensor pipe
 // 81-86 % active; back to back under the power cap 110 us.
@@ -406,7 +406,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------
-// CTA pairs (M > 128): a cluster of two CTAs computes 256 x 256 accumulators
+// CTA pairs: a cluster of two CTAs computes 256 x 256 accumulators
 // with tcgen05.mma.cta_group::2 (M = 256, N = 256, K = 64) issued by the even
 // CTA.  Per K block a CTA loads its 128 rows of A and 128 of B's 256 rows, 32 KB
 // instead of the single CTA's 48 KB, and its tensor core reads 8 KB instead of
@@ -754,7 +754,12 @@ static int launch_gemm(const void* A, const void* B, const void* B2, GemmParams 
     const uint64_t group = GROUP_A_BYTES / ((uint64_t)BM * row);
     p.group_m = (int)(group < 1 ? 1 : group > 64 ? 64 : group);
     const int tiles_n = ceil_div(p.N, ACT >= 0 ? BN / 2 : BN);
-    if (p.M > BM) {
+    // Pairs above 128 rows, unless one wave of single CTAs does it with a short K, where
+    // a pair's longer start shows (us, single / pairs: 160x4096x1024 5.6 / 6.5,
+    // 512x8192x2048 7.7 / 8.7, 1024x4096x4096 10.8 / 11.2, 512x4096x4096 10.4 / 10.1,
+    // 512x8192x8192 18.0 / 16.6).
+    const int64_t singles = (int64_t)ceil_div(p.M, BM) * tiles_n;
+    if (p.M > BM && (singles > info->sm_count || p.K > 16 * BK)) {
         QG_CUDA(cudaFuncSetAttribute(gemm_mxfp4_pair_kernel<OUT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      P_SMEM_BYTES));
         int pairs = 0;
@@ -767,8 +772,7 @@ static int launch_gemm(const void* A, const void* B, const void* B2, GemmParams 
         return QG_OK;
     }
     QG_CUDA(cudaFuncSetAttribute(gemm_mxfp4_kernel<OUT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
-    const int64_t tiles = (int64_t)ceil_div(p.M, BM) * tiles_n;
-    const int grid = tiles < info->sm_count ? (int)tiles : info->sm_count;
+    const int grid = singles < info->sm_count ? (int)singles : info->sm_count;
     QG_CUDA(launch_overlapped(gemm_mxfp4_kernel<OUT, ACT>, dim3(grid), dim3(GEMM_THREADS), SMEM_BYTES, stream, 1, tmA, tmB,
                               tmB2, p));
     return QG_OK;
@@ -789,13 +793,16 @@ static int check_mx(const char* name, const void* A, const void* SFA, const void
 
 } // namespace mx
 
-// Which kernel: the one for few rows up to 64 rows (32 of a gated product, whose
-// tiles are half as wide), and while 128 x 256 tiles would leave half of the SMs
-// idle; then single CTAs up to 128 rows, pairs above.  Measured at K=8192, few
-// rows / single / pairs: 64x28672 24.6 / 25.6 / 30.3 us, 128x28672 28.2 / 27.8 /
-// 33.2; gated at K=4096: 64x14336 16.5 / 15.5 / 19.5, 128x14336 19.0 / 16.7 / 20.4.
-static bool use_rows(int M, int cols, bool is_gated) {
-    return M <= (is_gated ? 32 : 64) || 2 * (int64_t)ceil_div(M, mx::BM) * ceil_div(cols, mx::BN) <= 148;
+// Whether the kernel for few rows takes it: up to 64 rows (32 of a gated product,
+// whose tiles are half as wide), and wherever it splits K four ways or more, which
+// pays for its own start and join.  Measured, few rows / single / pairs: 64x28672x8192
+// 24.6 / 25.6 / 30.3 us, 128x28672x8192 28.2 / 27.8 / 33.2; 256x1024x8192 (split in
+// eight) 8.8 / 14.9 / 14.2, 256x4096x4096 (four) 9.1 / 9.7 / 9.9, 192x8192x8192 (one)
+// 16.7 / 17.9 / 15.9, 512x4096x14336 (two) 21.4 / - / 22.4, 256x4096x1024 (one) 7.1 /
+// 5.6 / 6.5; gated 64x14336x4096 16.5 / 15.5 / 19.5, 128x14336x4096 19.0 /
+// 16.7 / 20.4.
+static bool use_rows(int M, int N, int K, bool is_gated) {
+    return M <= (is_gated ? 32 : 64) || mx::rows_split(M, N, K, is_gated) >= 4;
 }
 
 int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, void* C, int out_type, int M, int N,
@@ -804,7 +811,7 @@ int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, v
     if (rc) return rc;
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFB), nullptr, C, nullptr,
                      nullptr, 1, false};
-    const bool few = use_rows(M, N, false);
+    const bool few = use_rows(M, N, K, false);
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)C % 2 == 0, "qg_gemm_mxfp4: C is not aligned to its element");
@@ -829,7 +836,7 @@ int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void*
     QG_CHECK_ARG(act == QG_ACT_SILU || act == QG_ACT_GELU_TANH, "qg_gemm_gated_mxfp4: unknown activation %d", act);
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFG),
                      static_cast<const uint8_t*>(SFU), H, static_cast<uint8_t*>(SFH), nullptr, 1, false};
-    const bool silu = act == QG_ACT_SILU, few = use_rows(M, 2 * N, true);
+    const bool silu = act == QG_ACT_SILU, few = use_rows(M, N, K, true);
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)H % 2 == 0, "qg_gemm_gated_mxfp4: H is not aligned to its element");

@@ -1,5 +1,5 @@
 // qg_gemm_mxfp4_rows.cu -- the products of qg_gemm_mxfp4.cu for few rows of A
-// (decode steps, short prompts), where reading the weights once is the whole
+// (decode steps, short prompts; more rows where a long K meets few tiles), where reading the weights once is the whole
 // cost: K (1/2 + 1/32) bytes per weight row against NT columns of arithmetic.
 //
 // The operands change places: a tile takes 128 weight rows as the M side of
@@ -391,21 +391,12 @@ static int launch_nt(const void* X, const void* W, const void* W2, Params p, int
     return QG_OK;
 }
 
+// Rows of A per tile.
+static int row_tile(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+
 template <int OUT, int ACT>
 static int launch(const void* X, const void* W, const void* W2, const Params& p, cudaStream_t stream) {
-    DeviceInfo* info = nullptr;
-    int rc = current_device_info(&info);
-    if (rc) return rc;
-    const int nk = (p.K + BK - 1) / BK;
-    const int nt = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
-    const int64_t tiles = (int64_t)ceil_div(p.N, ACT >= 0 ? BW / 2 : BW) * ceil_div(p.M, nt);
-    // As many CTAs as one wave holds (two per SM), four K blocks each at least: a
-    // CTA's start and end cost 2-3 us, which a second wave pays again, and the join
-    // grows with the split.  Measured (one row, K=8192): N=28672 22.8 us unsplit, 26.1
-    // in two, 31.5 in four; N=8192 14.1, 10.7, 10.4 and 13.9 in eight; N=1024 13.3, 8.6,
-    // 6.2, 5.1.  333 x 1001 x 4128 (17 blocks): 7.4 in four, 9.6 in eight.
-    int split = 1;
-    while (split < 8 && 2 * split * tiles <= 2 * info->sm_count && 8 * split <= nk) split *= 2;
+    const int nt = row_tile(p.M), split = rows_split(p.M, p.N, p.K, ACT >= 0);
     switch (nt) {
         case 16: return launch_nt<16, OUT, ACT>(X, W, W2, p, split, stream);
         case 32: return launch_nt<32, OUT, ACT>(X, W, W2, p, split, stream);
@@ -415,6 +406,20 @@ static int launch(const void* X, const void* W, const void* W2, const Params& p,
 }
 
 } // namespace rows
+
+int rows_split(int M, int N, int K, bool is_gated) {
+    using namespace rows;
+    const int nk = (K + BK - 1) / BK;
+    const int64_t tiles = (int64_t)ceil_div(N, is_gated ? BW / 2 : BW) * ceil_div(M, row_tile(M));
+    // As many CTAs as one wave holds (two per SM of 148), four K blocks each at least:
+    // a CTA's start and end cost 2-3 us, which a second wave pays again, and the join
+    // grows with the split.  Measured (one row, K=8192): N=28672 22.8 us unsplit, 26.1
+    // in two, 31.5 in four; N=8192 14.1, 10.7, 10.4 and 13.9 in eight; N=1024 13.3, 8.6,
+    // 6.2, 5.1.  333 x 1001 x 4128 (17 blocks): 7.4 in four, 9.6 in eight.
+    int split = 1;
+    while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= nk) split *= 2;
+    return split;
+}
 
 int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,
               void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream) {
