@@ -83,6 +83,12 @@ int rows_split(int M, int N, int K, bool is_gated);
 int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,
               void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream);
 }
+namespace ffn {
+// The same for the gated product of 16-bit operands (qg_gemm_gated_rows.cu); G and U null or kept.
+int rows_split(int M, int N, int K);
+int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
+               int N, int K, cudaStream_t stream);
+}
 int gen_w4a16(void* X, void* W, void* S, void* Z, int M, int N, int K, uint64_t seed, uint32_t tid0, cudaStream_t s);
 uint64_t gemv_w4a16_workspace_bytes(int M, int N, int K, int sm_count);
 // `chk.expect` (when set) is the golden output, compared word for word by the writer of each output.

@@ -7,6 +7,8 @@
 #pragma once
 
 #include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "../../include/pantheon_qgemm.h"
@@ -45,5 +47,26 @@ __device__ __forceinline__ void gate_slope(float g, float& a, float& s) {
     a = g * p;
     s = fmaf(c * p * (1.0f - p), dy, p);
 }
+
+// Two values of a 16-bit type in a word, rounded to nearest even.
+template <typename T> struct Pack;
+template <> struct Pack<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t two(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) {
+        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+    }
+};
+template <> struct Pack<__half> {
+    static __device__ __forceinline__ uint32_t two(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    }
+};
 
 } // namespace qg

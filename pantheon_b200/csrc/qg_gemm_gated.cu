@@ -33,6 +33,7 @@
 // that rounding is gone; such calls last as long as their launches.  With more
 // values the second term's products would count (16x8192x4096: dX 80 us for 45).
 // G and U as kept are rounded likewise; H comes from the unrounded sums.
+// Few rows have a forward kernel of their own (use_rows, qg_gemm_gated_rows.cu).
 // Bound by the tensor cores: measured at 4096x8192x4096 bf16 the forward pass takes
 // 342-349 us (1.58-1.61 PFLOP/s, 0.93-0.94 of the measured rate, tensor pipe 96 %
 // active), the backward pass 740-760 us (47 of them the stream over M x N, the rest at
@@ -218,38 +219,6 @@ __device__ __forceinline__ void umma_commit_both(uint64_t* bar, uint32_t pair_in
                  ::"r"(smem_u32(bar)), "h"((uint16_t)(3u << (2 * pair_in_cluster))) : "memory");
 }
 
-__device__ __forceinline__ uint32_t cluster_nctas() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
-template <typename T> struct Pack;
-template <> struct Pack<__nv_bfloat16> {
-    static __device__ __forceinline__ uint32_t two(float a, float b) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    static __device__ __forceinline__ float2 unpack(uint32_t w) {
-        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-    }
-};
-template <> struct Pack<__half> {
-    static __device__ __forceinline__ uint32_t two(float a, float b) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    static __device__ __forceinline__ float2 unpack(uint32_t w) {
-        return __half22float2(*reinterpret_cast<const __half2*>(&w));
-    }
-};
-
 template <typename T>
 __device__ __forceinline__ void store32(void* out, int row0, const Tile& tl, int n0, const float (&f)[32]) {
     uint4 v[4];
@@ -306,7 +275,7 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
     const uint32_t rank = crank & 1u, sub = crank >> 1;     // CTA of the pair, pair of the cluster
     const uint32_t leader_cta = crank & ~1u;
     const bool leader = rank == 0;
-    const int subs = SPLIT ? (int)(cluster_nctas() >> 1) : 1;
+    const int subs = SPLIT ? (int)(cluster_size() >> 1) : 1;
     const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
     const int cluster = (int)blockIdx.x / (2 * subs);       // SPLIT: all that the pairs do is in here
     const bool parted = SPLIT && cluster < p.whole_from;    // and whether it is a part of a tile
@@ -625,13 +594,15 @@ static int launch_kernel(const Maps& maps, Params p, int subs, const DeviceInfo*
 // Pairs per tile, of `units` tiles and `nk` blocks in the longest: 4 or 2 while all
 // the clusters fit at once and the contraction is long enough.  Joining the parts
 // costs about 4.5 us (128 KB per CTA over distributed shared memory), a block
-// 0.3 us: with 16 blocks a split loses (1x1024x1024 9.8 us against 8.9), with 32 and
-// more it wins (256x2048x2048 14.5 against 17.1, 64x1024x4096 14.9 against 24.0).
-constexpr int SPLIT_MIN_BLOCKS = 20;
+// 0.3 us.  Forward (where use_rows leaves it: two pairs), split / whole:
+// 512x2048x1280 (20 blocks) 12.5 / 11.0 us, 512x2048x2048 (32) 14.6 / 14.6,
+// 256x4096x4096 (64) 20.6 / 24.1.  Backward: 256x768x512 (24) 13.4 / 12.7,
+// 2000x256x1024 (32) 14.7 / 15.6, 512x960x1024 (30) 14.1 / 15.1.
+constexpr int split_min_blocks(bool back) { return back ? 20 : 32; }
 template <typename T, bool BACK, int ACT>
 static int pick_split(int* out, int64_t units, int nk, const DeviceInfo* info) {
     *out = 1;
-    for (int s = 2; s <= MAX_SPLIT && nk >= SPLIT_MIN_BLOCKS; s *= 2) {
+    for (int s = 2; s <= MAX_SPLIT && nk >= split_min_blocks(BACK); s *= 2) {
         int clusters = 0;
         const int rc = resident_clusters(gated_kernel<T, BACK, ACT, true, 1>, 2 * s, &clusters, info);
         if (rc) return rc;
@@ -665,6 +636,13 @@ static int check_shape(const char* name, int M, int N, int K) {
 // Terms of dG and dU (see the head of this file).
 static int grad_parts(int M, int N) { return (int64_t)M * N <= 65536 ? 2 : 1; }
 
+// Whether the kernel for few rows takes the forward pass: up to 64 rows, and wherever
+// it splits K four ways or more.  Measured (pairs / few rows, us): 1x1024x1024 8.7 /
+// 3.8, 64x1024x4096 14.1 / 7.9, 64x8192x4096 28.9 / 25.7, 128x8192x4096 (unsplit) 29.9 /
+// 30.5, 128x4096x4096 (four) 20.3 / 17.9, 256x4096x4096 (two) 20.3 / 23.3, 256x1024x1024
+// (four) 10.3 / 7.0, 512x1024x4096 (four) 18.1 / 14.6, 1024x1024x4096 (two) 19.5 / 21.6.
+static bool use_rows(int M, int N, int K) { return M <= 64 || rows_split(M, N, K) >= 4; }
+
 template <typename T>
 static int forward(const char* name, const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, int act,
                    int M, int N, int K, cudaStream_t stream) {
@@ -675,6 +653,7 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
     if (rc) return rc;
     QG_CHECK_ARG((((uintptr_t)X | (uintptr_t)Wg | (uintptr_t)Wu | (uintptr_t)H | (uintptr_t)G | (uintptr_t)U) & 15) == 0,
                  "%s: operands and outputs must be 16-byte aligned", name);
+    if (use_rows(M, N, K)) return gated_rows(X, Wg, Wu, H, G, U, std::is_same<T, __half>::value, act, M, N, K, stream);
     Maps maps;
     if ((rc = make_map(&maps.x, X, M, K, BM)) || (rc = make_map(&maps.wg, Wg, N, K, 128)) ||
         (rc = make_map(&maps.wu, Wu, N, K, 128)))

@@ -27,6 +27,7 @@
 #include "qg_launch.cuh"
 #include "qg_mxfp4.cuh"
 #include "qg_mxfp4_mma.cuh"
+#include "qg_rows.cuh"
 
 #include <cuda_bf16.h>
 
@@ -83,23 +84,6 @@ struct Barriers {
     uint32_t tmem_base;
     int abort;
 };
-
-__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
 
 template <int NT, int OUT, int ACT>   // ACT < 0: the plain product
 __global__ void __launch_bounds__(THREADS, 2)

@@ -2,7 +2,7 @@
 // (TMEM's layout), so a lane's 16-byte stores meet 31 other rows in one
 // instruction: 32 lines, a clock each.  Exchanged among four (eight) neighbouring
 // lanes first, each instruction writes 64 (128) contiguous bytes of eight (four)
-// rows instead.
+// rows instead.  And reads of other CTAs' partial rows over distributed shared memory.
 #pragma once
 
 #include <cstdint>
@@ -59,6 +59,28 @@ __device__ __forceinline__ void store_rows(E* out, int row0, int rows, int n0, i
                 }
         }
     }
+}
+
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
 }
 
 } // namespace qg

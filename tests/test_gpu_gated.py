@@ -81,6 +81,24 @@ def test_forward_matches_the_definition(cuda_device, shape, act, kind):
     assert pb.device_status(0) == 0
 
 
+# the kernel for few rows: each of its tiles, whole and with K in two to eight parts, one row tile and
+# several; and two pairs of CTAs to a tile, whose shapes lie beside those
+FEW = [(1, 8, 4104), (1, 9608, 264), (16, 1000, 520), (17, 136, 1032), (32, 72, 2056), (33, 72, 520), (64, 5000, 264),
+       (65, 264, 1032), (129, 136, 4104), (300, 1000, 2056), (300, 1608, 2120), (513, 1032, 2056)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", FEW, ids=lambda s: "x".join(map(str, s)))
+def test_forward_of_few_rows(cuda_device, shape, kind):
+    x, wg, wu = _inputs(shape, kind, cuda_device)
+    act = ACTS[shape[0] % 2]
+    f = TYPES[kind][3]
+    h, g, u = f(x, wg, wu, act=act, keep=True)
+    _check_forward(x, wg, wu, act, kind, h, g, u)
+    assert torch.equal(f(x, wg, wu, act=act), h)
+    assert pb.device_status(0) == 0
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
