@@ -62,19 +62,21 @@ def act_arg(g, act):
     return g if act == 0 else 2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)
 
 
+def _logistic(g, act):
+    """p = 1 / (1 + exp(-y)).  For gelu this is 0.5 (1 + tanh(y / 2)), whose sum would cancel: at
+    y = -36 it is 1.6e-16, and 64-bit numbers just below 1 are 1.1e-16 apart."""
+    with np.errstate(over="ignore"):
+        return 1 / (1 + np.exp(-act_arg(g, act)))
+
+
 def activation(g, act):
-    if act == 0:
-        return g / (1 + np.exp(-g))
-    return 0.5 * g * (1 + np.tanh(np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)))
+    return g * _logistic(g, act)
 
 
 def slope(g, act):
-    if act == 0:
-        p = 1 / (1 + np.exp(-g))
-        return p * (1 + g * (1 - p))
-    z = np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)
-    t = np.tanh(z)
-    return 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * np.sqrt(2 / np.pi) * (1 + 3 * 0.044715 * g ** 2)
+    p = _logistic(g, act)
+    dy = 1 if act == 0 else 2 * np.sqrt(2 / np.pi) * (1 + 3 * 0.044715 * g ** 2)
+    return p + g * p * _logistic(-g, act) * dy
 
 
 def sum_bound(a, b):
