@@ -84,10 +84,15 @@ int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, co
               void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream);
 }
 namespace ffn {
-// The same for the gated product of 16-bit operands (qg_gemm_gated_rows.cu); G and U null or kept.
+// The forward pass and dX of the gated block of 16-bit operands for few rows of X
+// (qg_gemm_gated_rows.cu): CTAs that share a tile's contraction, and the launches.
+// G and U null or kept; d = dG, dU and their remainders (null: none).
 int rows_split(int M, int N, int K);
+int rows_split_dx(int M, int N, int K);
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
                int N, int K, cudaStream_t stream);
+int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,
+                  cudaStream_t stream);
 }
 int gen_w4a16(void* X, void* W, void* S, void* Z, int M, int N, int K, uint64_t seed, uint32_t tid0, cudaStream_t s);
 uint64_t gemv_w4a16_workspace_bytes(int M, int N, int K, int sm_count);

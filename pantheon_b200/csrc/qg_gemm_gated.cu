@@ -5,7 +5,8 @@
 //   backward   dG = dH * U * act'(G), dU = dH * act(G)    (a stream over M x N)
 //              dX = dG Wg + dU Wu                          (contraction over 2 N)
 //              dWg = dG^T X, dWu = dU^T X                  (contraction over M)
-//                                                          (one kernel for the three)
+//                                                          (one kernel for the three,
+//                                                           or dX apart with few rows)
 //
 // Each product is tiles of CTA pairs (256 x 256 accumulators, tcgen05.mma
 // .cta_group::2 M=256 N=256 K=16 issued by the even CTA); per 64-deep contraction
@@ -31,9 +32,10 @@
 // few values (M N <= 65536), a handful of which can carry a sum, they go as two
 // terms (value and remainder; a stage then holds both beside one block of B) and
 // that rounding is gone; such calls last as long as their launches.  With more
-// values the second term's products would count (16x8192x4096: dX 80 us for 45).
+// values the second term would double the products' time.
 // G and U as kept are rounded likewise; H comes from the unrounded sums.
-// Few rows have a forward kernel of their own (use_rows, qg_gemm_gated_rows.cu).
+// Few rows have a kernel of their own for forward and dX (use_rows, use_rows_dx,
+// qg_gemm_gated_rows.cu).
 // Bound by the tensor cores: measured at 4096x8192x4096 bf16 the forward pass takes
 // 342-349 us (1.58-1.61 PFLOP/s, 0.93-0.94 of the measured rate, tensor pipe 96 %
 // active), the backward pass 740-760 us (47 of them the stream over M x N, the rest at
@@ -185,20 +187,6 @@ __device__ __forceinline__ int cluster_tile(int c, int sub, int subs, const Para
 __device__ __forceinline__ int part_begin(int nk, int sub, int subs) {
     const int n = min(subs, nk);
     return sub >= n ? nk : (int)((int64_t)nk * sub / n);
-}
-
-// Descriptor of an MN-major operand tile: blocks of 64 elements (128 bytes)
-// along MN x BK contraction rows of 128 bytes each, 128-byte swizzled as TMA
-// stores them.  LBO = bytes from one 64-element block to the next, SBO = bytes
-// between groups of eight contraction rows.
-__device__ __forceinline__ uint64_t make_sdesc_mnmajor_sw128(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-    d |= (uint64_t)((uint32_t)MN_BLOCK >> 4) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1u << 46;
-    d |= (uint64_t)2u << 61;
-    return d;
 }
 
 // 128 rows of an operand: K-major in one box, MN-major in two side by side.
@@ -368,8 +356,8 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
             const int i0 = parted ? part_begin(tl.nk, (int)sub, subs) : 0, i1 = parted ? part_begin(tl.nk, (int)sub + 1, subs) : tl.nk;
             auto blocks = [&](auto a_major) {
                 constexpr bool A_IS_MN = decltype(a_major)::value;
-                const uint64_t a_desc = A_IS_MN ? make_sdesc_mnmajor_sw128(a_addr) : make_sdesc_kmajor_sw128(a_addr);
-                const uint64_t b_desc = BACK ? make_sdesc_mnmajor_sw128(b_addr) : make_sdesc_kmajor_sw128(b_addr);
+                const uint64_t a_desc = A_IS_MN ? make_sdesc_mnmajor_sw128(a_addr, MN_BLOCK) : make_sdesc_kmajor_sw128(a_addr);
+                const uint64_t b_desc = BACK ? make_sdesc_mnmajor_sw128(b_addr, MN_BLOCK) : make_sdesc_kmajor_sw128(b_addr);
                 // 16 contraction elements: 32 bytes of a K-major row, 16 rows of an MN-major tile
                 constexpr uint32_t A_STEP = A_IS_MN ? UMMA_K * 128 >> 4 : UMMA_K * 2 >> 4;
                 constexpr uint32_t B_STEP = BACK ? UMMA_K * 128 >> 4 : UMMA_K * 2 >> 4;
@@ -642,6 +630,14 @@ static int grad_parts(int M, int N) { return (int64_t)M * N <= 65536 ? 2 : 1; }
 // 30.5, 128x4096x4096 (four) 20.3 / 17.9, 256x4096x4096 (two) 20.3 / 23.3, 256x1024x1024
 // (four) 10.3 / 7.0, 512x1024x4096 (four) 18.1 / 14.6, 1024x1024x4096 (two) 19.5 / 21.6.
 static bool use_rows(int M, int N, int K) { return M <= 64 || rows_split(M, N, K) >= 4; }
+// And dX, in a launch apart from dWg's and dWu's: more rows only where its contraction
+// is long enough to outweigh that.  All gradients, in one launch / with dX apart:
+// 1x8192x4096 109 / 62 us, 16x8192x4096 78 / 61, 64x1024x4096 25.6 / 18.3, 64x512x512
+// 15.0 / 12.2, 128x1024x512 13.5 / 13.1, 256x4096x1024 31.1 / 25.3, 512x8192x512 45.5 /
+// 36.6; 256x1024x1024 14.5 / 16.2, 512x2048x512 17.8 / 20.5, 1024x512x512 11.4 / 17.6.
+static bool use_rows_dx(int M, int N, int K) {
+    return M <= 64 || (rows_split_dx(M, N, K) >= 4 && M <= 5 * 2 * ceil_div(N, BK));
+}
 
 template <typename T>
 static int forward(const char* name, const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, int act,
@@ -666,14 +662,18 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
                               : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
 }
 
-// The three products of the backward pass.
+// The products of the backward pass (dx_apart: dWg and dWu).
 template <typename T, int PARTS>
-static int products(const Maps& maps, void* dX, void* dWg, void* dWu, int M, int N, int K, const DeviceInfo* info,
-                    cudaStream_t stream) {
+static int products(const Maps& maps, bool dx_apart, void* dX, void* dWg, void* dWu, int M, int N, int K,
+                    const DeviceInfo* info, cudaStream_t stream) {
     int rc;
     const int nk_dx = 2 * ceil_div(N, BK), nk_dw = ceil_div(M, BK);
     const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
     const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
+    if (dx_apart) {
+        const Params p{M, N, K, 0, 1, 0, 0, 1, 1, 0, 1, nullptr, dWg, dWu, nullptr};
+        return launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units_dw, nk_dw, stream);
+    }
     // One launch for the three: all tiles split; or the long ones, where they are few of
     // many blocks beside many of few (dX with few rows of X, dWg and dWu with many) and
     // all fit at once; or none split.  Where the long ones should be split and do not
@@ -739,6 +739,13 @@ static int backward(const char* name, const void* dH, const void* X, const void*
                              : (silu ? gate_backward_kernel<T, QG_ACT_SILU, 1> : gate_backward_kernel<T, QG_ACT_GELU_TANH, 1>);
     QG_CUDA(launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, 1, vh, vg, vu,
                               static_cast<uint4*>(workspace), n8));
+    const bool dx_apart = use_rows_dx(M, N, K);
+    if (dx_apart && dX) {
+        const void* d[4] = {};
+        for (int i = 0; i < 2 * parts; ++i) d[i] = static_cast<const uint8_t*>(workspace) + i * one;
+        if ((rc = gated_rows_dx(d, Wg, Wu, dX, std::is_same<T, __half>::value, M, N, K, stream))) return rc;
+    }
+    if (dx_apart && !dWg) return QG_OK;
     Maps maps;
     for (int w = 0; w < 2; ++w) {
         for (int q = 0; q < parts; ++q) {
@@ -752,8 +759,8 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     }
     if ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)) || (rc = make_map(&maps.x, X, M, K, BK)))
         return rc;
-    return parts == 2 ? products<T, 2>(maps, dX, dWg, dWu, M, N, K, info, stream)
-                      : products<T, 1>(maps, dX, dWg, dWu, M, N, K, info, stream);
+    return parts == 2 ? products<T, 2>(maps, dx_apart, dX, dWg, dWu, M, N, K, info, stream)
+                      : products<T, 1>(maps, dx_apart, dX, dWg, dWu, M, N, K, info, stream);
 }
 
 } // namespace ffn

@@ -1,18 +1,23 @@
-// qg_gemm_gated_rows.cu -- the forward pass of qg_gemm_gated.cu for few rows of X
-// (decode steps, short prompts; more rows where a long K meets few tiles), where
-// reading the weights once is the whole cost: 4 N K bytes.
+// qg_gemm_gated_rows.cu -- the forward pass and dX of qg_gemm_gated.cu for few rows
+// of X (decode steps, short prompts; more rows where a long contraction meets few
+// tiles), where reading the weights once is the whole cost: 4 N K bytes.
 //
-// As in qg_gemm_mxfp4_rows.cu the operands change places: a tile takes 64 rows of
-// Wg and the same 64 of Wu as the M side of tcgen05.mma and NT = 16, 32, 64 or
-// 128 rows of X as its N side.  K is split over the CTAs of a cluster (1 to 8);
-// each sums its part in TMEM, puts the partial tile in its shared memory, and
-// every CTA of the cluster joins a share of the rows from all of them over
+// As in qg_gemm_mxfp4_rows.cu the operands change places: the weights are the M
+// side of tcgen05.mma, 128 to a tile, and NT = 16, 32, 64 or 128 rows of X (dG, dU)
+// its N side.  The contraction is split over the CTAs of a cluster (1 to 8); each
+// sums its part in TMEM, puts the partial tile in its shared memory, and every
+// CTA of the cluster joins a share of the rows from all of them over
 // distributed shared memory, in rank order: no workspace, no atomics, the same
 // bits on every run.
+//   forward   a tile's weights are 64 rows of Wg and the same 64 of Wu
+//   dX        128 columns of Wg, then of Wu along the contraction (2 N): the weights
+//             are read MN-major.  dG and dU in two terms (PARTS) bring their
+//             remainders beside them in a stage.
 //
 // Bound by the weights' bytes: measured (bf16) 1x8192x4096 22.7 us (134 MB, 5.9 TB/s,
 // 0.90 of the measured copy bandwidth), 16x8192x4096 23.7, 64x8192x4096 25.7,
-// 1x4096x4096 13.4, 1x1024x1024 3.8.  What is left is a launch's start and end, 2-3 us.
+// 1x4096x4096 13.4, 1x1024x1024 3.8; dX 1x8192x4096 26.0 with its stream over M x N,
+// 64x8192x4096 28.4.  What is left is a launch's start and end, 2-3 us.
 //
 // 192 threads, two CTAs per SM:
 //   warp 0      producer: TMA loads per 64-element K block, into a ring of up to 105 KB.
@@ -34,18 +39,19 @@ namespace rows {
 
 using mx::warp_wait;
 
-constexpr int BW = 128;                        // weight rows of a tile: TN of Wg, TN of Wu
-constexpr int TN = BW / 2;                     // output columns of a tile
+constexpr int BW = 128;                        // weight rows (dX: columns) of a tile
 constexpr int BK = 64;
 constexpr int BK_BYTES = BK * 2;
 constexpr int UMMA_K = 16;
 constexpr int W_BYTES = BW * BK_BYTES;         // 16 KB
 constexpr int THREADS = 192;
 
-template <int NT>
+constexpr int DX = -1;                         // in place of the activation
+
+template <int NT, int PARTS>
 struct Cfg {
-    static constexpr int X_BYTES = NT * BK_BYTES;
-    static constexpr int STAGE = W_BYTES + X_BYTES;
+    static constexpr int X_BYTES = NT * BK_BYTES;           // of one term
+    static constexpr int STAGE = W_BYTES + PARTS * X_BYTES;
     static constexpr int STAGES = 105 * 1024 / STAGE;       // two CTAs share an SM's 227 KB
     static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
     static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
@@ -56,9 +62,14 @@ constexpr uint32_t SITE_PRODUCER = 0x00090001u;
 constexpr uint32_t SITE_MMA_FULL = 0x00090002u;
 constexpr uint32_t SITE_EPI = 0x00090003u;
 
+struct Maps {
+    CUtensorMap w[2];         // Wg, Wu
+    CUtensorMap x[2][2];      // X; dX: [dG, dU][value, remainder]
+};
+
 struct Params {
     int M, N, K;
-    void* H;
+    void* out;                // H, or dX
     void* G;                  // or null
     void* U;
     DeviceStatus* status;
@@ -74,11 +85,12 @@ struct Barriers {
     int abort;
 };
 
-template <typename T, int NT, int ACT>
+template <typename T, int NT, int ACT, int PARTS>
 __global__ void __launch_bounds__(THREADS, 2)
-gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG,
-                  const __grid_constant__ CUtensorMap tmU, Params p) {
-    using C = Cfg<NT>;
+gated_rows_kernel(const __grid_constant__ Maps maps, Params p) {
+    constexpr bool BACK = ACT == DX;
+    using C = Cfg<NT, PARTS>;
+    constexpr int TN = BACK ? BW : BW / 2;           // output columns of a tile
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -93,7 +105,8 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
     const int n_tile = (int)(blockIdx.x / ranks) * TN;
     const int m0 = blockIdx.y * NT;
-    const int nk_all = (p.K + BK - 1) / BK;
+    const int half = ((BACK ? p.N : p.K) + BK - 1) / BK;     // dX: blocks of dG, as many of dU
+    const int nk_all = BACK ? 2 * half : half;
     const int kb0 = (int)((int64_t)nk_all * rank / ranks), kb1 = (int)((int64_t)nk_all * (rank + 1) / ranks);
 
     if (threadIdx.x == 0) {
@@ -116,7 +129,7 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     const uint32_t tmem_base = bars->tmem_base;
     volatile int* abort_flag = &bars->abort;
     wait_previous_grid();
-    float* part = reinterpret_cast<float*>(smem);    // [row of X][64 of G, 64 of U], over the ring once it is drained
+    float* part = reinterpret_cast<float*>(smem);    // [row][tile's weights], over the ring once it is drained
 
     if (warp == 0 && lane == 0) {
         // ------------------------------------------------------------ producer
@@ -127,9 +140,18 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
             uint64_t* full = &bars->full[stage];
             mbar_arrive_expect_tx(full, C::STAGE);
             uint8_t* w = sW + stage * W_BYTES;
-            tma_load_2d(w, &tmG, full, kb * BK_BYTES, n_tile);
-            tma_load_2d(w + W_BYTES / 2, &tmU, full, kb * BK_BYTES, n_tile);
-            tma_load_2d(sX + stage * C::X_BYTES, &tmX, full, kb * BK_BYTES, m0);
+            uint8_t* x = sX + stage * PARTS * C::X_BYTES;
+            if constexpr (BACK) {
+                const int which = kb >= half, b = kb - which * half;
+                tma_load_2d(w, &maps.w[which], full, n_tile * 2, b * BK);
+                tma_load_2d(w + W_BYTES / 2, &maps.w[which], full, n_tile * 2 + 128, b * BK);
+                for (int q = 0; q < PARTS; ++q)
+                    tma_load_2d(x + q * C::X_BYTES, &maps.x[which][q], full, b * BK_BYTES, m0);
+            } else {
+                tma_load_2d(w, &maps.w[0], full, kb * BK_BYTES, n_tile);
+                tma_load_2d(w + W_BYTES / 2, &maps.w[1], full, kb * BK_BYTES, n_tile);
+                tma_load_2d(x, &maps.x[0][0], full, kb * BK_BYTES, m0);
+            }
             armed |= 1u << stage;
             armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
             if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
@@ -145,18 +167,23 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     } else if (warp == 1 && lane == 0) {
         // ------------------------------------------------------------ MMA issuer
         constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
-        constexpr uint32_t IDESC = make_idesc(1, FMT, FMT, BW, NT);
+        constexpr uint32_t IDESC = make_idesc(1, FMT, FMT, BW, NT) | (BACK ? 1u << 15 : 0u);
         uint32_t stage = 0, phase = 0;
         bool ok = true, issued = false;
         for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait(&bars->full[stage], phase, abort_flag, p.status, SITE_MMA_FULL)) { ok = false; break; }
             tc_fence_after();
             const uint32_t w_addr = smem_u32(sW + stage * W_BYTES);
-            const uint32_t x_addr = smem_u32(sX + stage * C::X_BYTES);
+            const uint32_t x_addr = smem_u32(sX + stage * PARTS * C::X_BYTES);
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k)
-                umma_f16(tmem_base, make_sdesc_kmajor_sw128(w_addr + k * (UMMA_K * 2)),
-                         make_sdesc_kmajor_sw128(x_addr + k * (UMMA_K * 2)), IDESC, kb != kb0 || k != 0 ? 1u : 0u);
+            for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k) {
+                    const uint64_t w_desc = BACK ? make_sdesc_mnmajor_sw128(w_addr + k * (UMMA_K * 128), W_BYTES / 2)
+                                                 : make_sdesc_kmajor_sw128(w_addr + k * (UMMA_K * 2));
+                    umma_f16(tmem_base, w_desc, make_sdesc_kmajor_sw128(x_addr + q * C::X_BYTES + k * (UMMA_K * 2)), IDESC,
+                             kb != kb0 || q != 0 || k != 0 ? 1u : 0u);
+                }
             issued = true;
             umma_commit(&bars->empty[stage]);
             if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
@@ -196,21 +223,32 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         // ------------------------------------------------------------ join and store: one row of X per warp and step
         const int mine = min(NT, p.M - m0);
         const uint32_t base = smem_u32(part);
-        const int n = n_tile + lane * 2;              // N is a multiple of 8
+        const int cols = BACK ? p.K : p.N;            // a multiple of 8
+        const int n = n_tile + lane * (BACK ? 4 : 2);
         for (int r = (int)rank + (int)ranks * (warp - 2); r < mine; r += (int)ranks * 4) {
-            float2 g = make_float2(0.0f, 0.0f), u = g;
-            for (uint32_t k = 0; k < ranks; ++k) {
-                const uint32_t at = mapa_shared(base + (uint32_t)(r * BW + lane * 2) * 4, k);
-                const float2 a = ld_cluster_v2(at), b = ld_cluster_v2(at + TN * 4);
-                g.x += a.x; g.y += a.y; u.x += b.x; u.y += b.y;
+            const size_t at = (size_t)(m0 + r) * cols + n;
+            if constexpr (BACK) {
+                float4 d = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (uint32_t k = 0; k < ranks; ++k) {
+                    const float4 v = ld_cluster_v4(mapa_shared(base + (uint32_t)(r * BW + lane * 4) * 4, k));
+                    d.x += v.x; d.y += v.y; d.z += v.z; d.w += v.w;
+                }
+                if (n < cols)
+                    static_cast<uint2*>(p.out)[at / 4] = make_uint2(Pack<T>::two(d.x, d.y), Pack<T>::two(d.z, d.w));
+            } else {
+                float2 g = make_float2(0.0f, 0.0f), u = g;
+                for (uint32_t k = 0; k < ranks; ++k) {
+                    const uint32_t from = mapa_shared(base + (uint32_t)(r * BW + lane * 2) * 4, k);
+                    const float2 a = ld_cluster_v2(from), b = ld_cluster_v2(from + TN * 4);
+                    g.x += a.x; g.y += a.y; u.x += b.x; u.y += b.y;
+                }
+                if (n >= cols) continue;
+                if (p.G) {
+                    static_cast<uint32_t*>(p.G)[at / 2] = Pack<T>::two(g.x, g.y);
+                    static_cast<uint32_t*>(p.U)[at / 2] = Pack<T>::two(u.x, u.y);
+                }
+                static_cast<uint32_t*>(p.out)[at / 2] = Pack<T>::two(gated<ACT, true>(g.x, u.x), gated<ACT, true>(g.y, u.y));
             }
-            if (n >= p.N) continue;
-            const size_t at = ((size_t)(m0 + r) * p.N + n) / 2;
-            if (p.G) {
-                static_cast<uint32_t*>(p.G)[at] = Pack<T>::two(g.x, g.y);
-                static_cast<uint32_t*>(p.U)[at] = Pack<T>::two(u.x, u.y);
-            }
-            static_cast<uint32_t*>(p.H)[at] = Pack<T>::two(gated<ACT, true>(g.x, u.x), gated<ACT, true>(g.y, u.y));
         }
     }
     cluster_sync();                                   // nobody leaves while its partial tile is being read
@@ -221,57 +259,78 @@ static int make_map(CUtensorMap* map, const void* base, int rows, int cols, int 
                         (uint64_t)cols * 2, BK_BYTES, (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int NT, int ACT>
-static int launch_nt(const void* X, const void* Wg, const void* Wu, Params p, int split, cudaStream_t stream) {
-    using C = Cfg<NT>;
-    int rc;
-    if ((rc = device_status_ptr(&p.status))) return rc;
-    CUtensorMap x, g, u;
-    if ((rc = make_map(&x, X, p.M, p.K, NT)) || (rc = make_map(&g, Wg, p.N, p.K, TN)) ||
-        (rc = make_map(&u, Wu, p.N, p.K, TN)))
-        return rc;
-    const auto kernel = gated_rows_kernel<T, NT, ACT>;
-    QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    QG_CUDA(launch_overlapped(kernel, dim3((unsigned)(ceil_div(p.N, TN) * split), (unsigned)ceil_div(p.M, NT)),
-                              dim3(THREADS), C::SMEM, stream, (unsigned)split, x, g, u, p));
-    return QG_OK;
-}
-
 // Rows of X per tile.
 static int row_tile(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
 
-template <typename T, int ACT>
-static int launch(const void* X, const void* Wg, const void* Wu, const Params& p, cudaStream_t stream) {
-    const int split = rows_split(p.M, p.N, p.K);
+// x: X, or for dX dG and dU, then their remainders.
+template <typename T, int NT, int ACT, int PARTS>
+static int launch_nt(const void* const (&x)[4], const void* Wg, const void* Wu, Params p, int split, cudaStream_t stream) {
+    constexpr bool BACK = ACT == DX;
+    using C = Cfg<NT, PARTS>;
+    int rc;
+    if ((rc = device_status_ptr(&p.status))) return rc;
+    Maps maps;
+    if ((rc = make_map(&maps.w[0], Wg, p.N, p.K, 64)) || (rc = make_map(&maps.w[1], Wu, p.N, p.K, 64))) return rc;
+    for (int i = 0; i < 4; ++i) {
+        if (!x[i]) maps.x[i & 1][i >> 1] = maps.x[0][0];      // not read
+        else if ((rc = make_map(&maps.x[i & 1][i >> 1], x[i], p.M, BACK ? p.N : p.K, NT))) return rc;
+    }
+    const auto kernel = gated_rows_kernel<T, NT, ACT, PARTS>;
+    QG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    const int tiles = BACK ? ceil_div(p.K, BW) : ceil_div(p.N, BW / 2);
+    QG_CUDA(launch_overlapped(kernel, dim3((unsigned)(tiles * split), (unsigned)ceil_div(p.M, NT)), dim3(THREADS),
+                              C::SMEM, stream, (unsigned)split, maps, p));
+    return QG_OK;
+}
+
+template <typename T, int ACT, int PARTS>
+static int launch(const void* const (&x)[4], const void* Wg, const void* Wu, const Params& p, int split,
+                  cudaStream_t stream) {
     switch (row_tile(p.M)) {
-        case 16: return launch_nt<T, 16, ACT>(X, Wg, Wu, p, split, stream);
-        case 32: return launch_nt<T, 32, ACT>(X, Wg, Wu, p, split, stream);
-        case 64: return launch_nt<T, 64, ACT>(X, Wg, Wu, p, split, stream);
-        default: return launch_nt<T, 128, ACT>(X, Wg, Wu, p, split, stream);
+        case 16: return launch_nt<T, 16, ACT, PARTS>(x, Wg, Wu, p, split, stream);
+        case 32: return launch_nt<T, 32, ACT, PARTS>(x, Wg, Wu, p, split, stream);
+        case 64: return launch_nt<T, 64, ACT, PARTS>(x, Wg, Wu, p, split, stream);
+        default: return launch_nt<T, 128, ACT, PARTS>(x, Wg, Wu, p, split, stream);
     }
 }
 
-} // namespace rows
-
 // As qg_gemm_mxfp4_rows.cu splits, whose blocks have as many bytes: one wave of two
-// CTAs per SM of 148, four K blocks each at least.
-int rows_split(int M, int N, int K) {
-    const int nk = ceil_div(K, rows::BK);
-    const int64_t tiles = (int64_t)ceil_div(N, rows::TN) * ceil_div(M, rows::row_tile(M));
+// CTAs per SM of 148, four blocks each at least.
+static int pick_split(int M, int tiles_n, int nk) {
+    const int64_t tiles = (int64_t)tiles_n * ceil_div(M, row_tile(M));
     int split = 1;
     while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= nk) split *= 2;
     return split;
 }
 
+} // namespace rows
+
+int rows_split(int M, int N, int K) { return rows::pick_split(M, ceil_div(N, rows::BW / 2), ceil_div(K, rows::BK)); }
+
+int rows_split_dx(int M, int N, int K) { return rows::pick_split(M, ceil_div(K, rows::BW), 2 * ceil_div(N, rows::BK)); }
+
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
                int N, int K, cudaStream_t stream) {
     const rows::Params p{M, N, K, H, G, U, nullptr};
+    const void* const x[4] = {X, nullptr, nullptr, nullptr};
+    const int split = rows_split(M, N, K);
     const bool silu = act == QG_ACT_SILU;
     if (half)
-        return silu ? rows::launch<__half, QG_ACT_SILU>(X, Wg, Wu, p, stream)
-                    : rows::launch<__half, QG_ACT_GELU_TANH>(X, Wg, Wu, p, stream);
-    return silu ? rows::launch<__nv_bfloat16, QG_ACT_SILU>(X, Wg, Wu, p, stream)
-                : rows::launch<__nv_bfloat16, QG_ACT_GELU_TANH>(X, Wg, Wu, p, stream);
+        return silu ? rows::launch<__half, QG_ACT_SILU, 1>(x, Wg, Wu, p, split, stream)
+                    : rows::launch<__half, QG_ACT_GELU_TANH, 1>(x, Wg, Wu, p, split, stream);
+    return silu ? rows::launch<__nv_bfloat16, QG_ACT_SILU, 1>(x, Wg, Wu, p, split, stream)
+                : rows::launch<__nv_bfloat16, QG_ACT_GELU_TANH, 1>(x, Wg, Wu, p, split, stream);
+}
+
+int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,
+                  cudaStream_t stream) {
+    const rows::Params p{M, N, K, dX, nullptr, nullptr, nullptr};
+    const int split = rows_split_dx(M, N, K);
+    if (d[2])
+        return half ? rows::launch<__half, rows::DX, 2>(d, Wg, Wu, p, split, stream)
+                    : rows::launch<__nv_bfloat16, rows::DX, 2>(d, Wg, Wu, p, split, stream);
+    return half ? rows::launch<__half, rows::DX, 1>(d, Wg, Wu, p, split, stream)
+                : rows::launch<__nv_bfloat16, rows::DX, 1>(d, Wg, Wu, p, split, stream);
 }
 
 } // namespace ffn

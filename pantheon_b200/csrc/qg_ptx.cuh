@@ -404,6 +404,13 @@ __device__ __forceinline__ uint64_t make_sdesc_kmajor_sw128(uint32_t smem_addr) 
     return d;
 }
 
+// The same of an MN-major operand tile: blocks of 64 two-byte elements (128 bytes)
+// along MN x 64 contraction rows of 128 bytes each.  LBO = `block` bytes from one
+// block to the next, SBO = 1024 bytes between groups of eight contraction rows.
+__device__ __forceinline__ uint64_t make_sdesc_mnmajor_sw128(uint32_t smem_addr, uint32_t block) {
+    return make_sdesc_kmajor_sw128(smem_addr) | (uint64_t)(block >> 4) << 16;
+}
+
 // Instruction descriptor, dense kinds (f16 / f8f6f4 / i8).  Bits: [4,6) D
 // format (1 = f32, 2 = s32), [7,10) A format, [10,13) B format, [15] A major,
 // [16] B major (0 = K), [17,23) N >> 3, [24,29) M >> 4.

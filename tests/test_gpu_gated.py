@@ -99,6 +99,27 @@ def test_forward_of_few_rows(cuda_device, shape, kind):
     assert pb.device_status(0) == 0
 
 
+# the same for dX, in one and two terms of dG and dU, with N inside a block of 64 and K inside a tile
+FEW_DX = [(1, 8, 8), (1, 4104, 136), (7, 9608, 264), (16, 520, 1000), (20, 1032, 136), (40, 3000, 72), (64, 264, 9608),
+          (65, 1032, 264), (100, 2056, 1000), (129, 4104, 136), (130, 264, 72), (1300, 520, 264), (2050, 520, 520),
+          (32, 4104, 72), (40, 1032, 136), (66, 520, 136), (300, 4104, 264)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", FEW_DX, ids=lambda s: "x".join(map(str, s)))
+def test_backward_of_few_rows(cuda_device, shape, kind):
+    x, wg, wu = _inputs(shape, kind, cuda_device)
+    forward, backward = TYPES[kind][3:]
+    act = ACTS[shape[0] % 2]
+    _, g, u = forward(x, wg, wu, act=act, keep=True)
+    dh = torch.randn(g.shape, device=cuda_device, generator=torch.Generator(cuda_device).manual_seed(6)).to(g.dtype)
+    got = backward(dh, x, wg, wu, g, u, act=act)
+    _check_backward(dh, x, wg, wu, g, u, act, kind, got)
+    assert torch.equal(backward(dh, x, wg, wu, g, u, act=act, need_dw=False)[0], got[0])
+    assert all(torch.equal(a, b) for a, b in zip(backward(dh, x, wg, wu, g, u, act=act, need_dx=False)[1:], got[1:]))
+    assert pb.device_status(0) == 0
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
