@@ -747,18 +747,18 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     }
     if (dx_apart && !dWg) return QG_OK;
     Maps maps;
-    for (int w = 0; w < 2; ++w) {
-        for (int q = 0; q < parts; ++q) {
+    if ((rc = make_map(&maps.x, X, M, K, BK))) return rc;
+    for (int w = 0; w < 2; ++w)
+        for (int q = 0; q < 2; ++q) {
             void* d = static_cast<uint8_t*>(workspace) + (2 * q + w) * one;
-            if ((rc = make_map(&maps.rows[w][q], d, M, N, BM)) || (rc = make_map(&maps.cols[w][q], d, M, N, BK))) return rc;
+            // (the second terms of one, and dX's operands where it is apart, are not read)
+            if (q >= parts) maps.cols[w][q] = maps.cols[w][0];
+            else if ((rc = make_map(&maps.cols[w][q], d, M, N, BK))) return rc;
+            if (q >= parts || dx_apart) maps.rows[w][q] = maps.cols[w][q];
+            else if ((rc = make_map(&maps.rows[w][q], d, M, N, BM))) return rc;
         }
-        if (parts == 1) {               // not read
-            maps.rows[w][1] = maps.rows[w][0];
-            maps.cols[w][1] = maps.cols[w][0];
-        }
-    }
-    if ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)) || (rc = make_map(&maps.x, X, M, K, BK)))
-        return rc;
+    maps.wg = maps.wu = maps.x;
+    if (!dx_apart && ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)))) return rc;
     return parts == 2 ? products<T, 2>(maps, dx_apart, dX, dWg, dWu, M, N, K, info, stream)
                       : products<T, 1>(maps, dx_apart, dX, dWg, dWu, M, N, K, info, stream);
 }

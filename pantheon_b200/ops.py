@@ -370,10 +370,10 @@ def gemm_gated_f16(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, act: int
 
 
 def gemm_gated_backward_workspace_bytes(M: int, N: int) -> int:
-    b = C.c_uint64()
-    check("qg_gemm_gated_backward_workspace_bytes",
-          load_library().qg_gemm_gated_backward_workspace_bytes(M, N, C.byref(b)))
-    return b.value
+    """Bytes of a gated block's backward workspace: dG and dU [M, N], in two terms up to 65536 values."""
+    if M <= 0 or N <= 0:
+        raise ValueError(f"gemm_gated_backward_workspace_bytes: empty shape {M}x{N}")
+    return (8 if M * N <= 65536 else 4) * M * N
 
 
 def gemm_gated_bf16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, G: torch.Tensor,

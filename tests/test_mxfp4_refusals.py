@@ -130,6 +130,16 @@ def test_gated_backward_refusals(qglib, name):
     _refused(f(P, P, P, P, P, P, P + 8, P, P, 0, 4, 8, 8, P, big, None), "aligned")
 
 
+def test_gated_workspace_bytes(qglib):
+    b = C.c_uint64()
+    for M, N in ((1, 8), (16, 4096), (16, 4104), (65536, 1), (65537, 1), (4096, 8192), (1 << 29, 1 << 29)):
+        assert qglib.qg_gemm_gated_backward_workspace_bytes(M, N, C.byref(b)) == 0
+        assert pb.gemm_gated_backward_workspace_bytes(M, N) == b.value
+    _refused(qglib.qg_gemm_gated_backward_workspace_bytes(0, 8, C.byref(b)), "workspace_bytes")
+    with pytest.raises(ValueError):
+        pb.gemm_gated_backward_workspace_bytes(4, 0)
+
+
 def test_gated_dense_refuses_cpu_tensors(qglib):
     x, w = torch.zeros((4, 8), dtype=torch.bfloat16), torch.zeros((8, 8), dtype=torch.bfloat16)
     with pytest.raises(ValueError):
