@@ -260,11 +260,12 @@ def test_offsets_past_32_bits(cuda_device):
     _check_backward(dh[-40:], x[-40:], wg, wu, gate[-40:], up[-40:], 0, "bf16", (dx[-40:], dwg, dwu))
 
 
-def test_captured_and_replayed_beside_an_eager_call(cuda_device):
-    x, wg, wu = _inputs((260, 264, 136), "bf16", cuda_device)
+@pytest.mark.parametrize("shape", [(260, 264, 136), (20, 1032, 136)], ids=lambda s: "x".join(map(str, s)))
+def test_captured_and_replayed_beside_an_eager_call(cuda_device, shape):
+    x, wg, wu = _inputs(shape, "bf16", cuda_device)
     _, g, u = pb.gemm_gated_bf16(x, wg, wu, keep=True)
     dh = torch.randn_like(g)
-    ws = torch.empty((pb.gemm_gated_backward_workspace_bytes(260, 264),), dtype=torch.uint8, device=cuda_device)
+    ws = torch.empty((pb.gemm_gated_backward_workspace_bytes(*shape[:2]),), dtype=torch.uint8, device=cuda_device)
 
     def step():
         h, g, u = pb.gemm_gated_bf16(x, wg, wu, keep=True)
