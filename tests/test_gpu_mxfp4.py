@@ -142,7 +142,7 @@ def test_gated_matches_the_definition(cuda_device, shape, act):
 # several, CTA pairs (more than 148 tiles, or K over 4096) with their last row tile in the first or
 # the second CTA and with several tiles each, and the kernel for few rows with K split on many rows
 WIDE = [(70, 19001, 288), (130, 10001, 544), (200, 5024, 1056), (513, 9999, 96), (1400, 4320, 800), (130, 9999, 4128),
-        (300, 1001, 4128), (130, 257, 8224)]
+        (300, 1001, 4128), (130, 257, 8224), (200, 5026, 1056), (520, 5004, 96), (1300, 2050, 224)]
 
 
 @pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32])
@@ -159,7 +159,7 @@ def test_wide_gemm_matches_the_definition(cuda_device, shape, out_type):
 
 @pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32, pb.QG_OUT_MXFP4])
 @pytest.mark.parametrize("shape", [(40, 9601, 288), (64, 9632, 352), (130, 5001, 544), (200, 4928, 1056), (513, 5024, 96),
-                                   (1400, 2176, 416), (200, 4928, 4128), (300, 480, 4128)], ids=lambda s: "x".join(map(str, s)))
+                                   (1400, 2176, 416), (200, 4928, 4128), (300, 480, 4128), (200, 5026, 96), (1400, 2179, 416)], ids=lambda s: "x".join(map(str, s)))
 def test_wide_gated_matches_the_definition(cuda_device, shape, out_type):
     M, N, K = shape
     if out_type == pb.QG_OUT_MXFP4 and N % 32:
