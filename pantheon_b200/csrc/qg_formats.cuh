@@ -77,18 +77,18 @@ int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, v
 int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void* SFG, const void* Wu, const void* SFU,
                      void* H, void* SFH, int out_type, int act, int M, int N, int K, cudaStream_t stream);
 namespace mx {
-// CTAs that the kernel for few rows gives K to, per tile.
-int rows_split(int M, int N, int K, bool is_gated);
-// Either product for few rows of A (qg_gemm_mxfp4_rows.cu); act < 0 is the plain one.  Arguments are checked by the caller.
+// Whether the kernel for few rows takes a product (qg_gemm_mxfp4_rows.cu), and its launch; act < 0
+// is the plain one.  Arguments are checked by the caller.
+bool use_rows(int M, int N, int K, bool is_gated);
 int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,
               void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream);
 }
 namespace ffn {
 // The forward pass and dX of the gated block of 16-bit operands for few rows of X
-// (qg_gemm_gated_rows.cu): CTAs that share a tile's contraction, and the launches.
-// G and U null or kept; d = dG, dU and their remainders (null: none).
-int rows_split(int M, int N, int K);
-int rows_split_dx(int M, int N, int K);
+// (qg_gemm_gated_rows.cu): whether that kernel takes them, and its launches.  G and U
+// null or kept; d = dG, dU and their remainders (null: none).
+bool use_rows(int M, int N, int K);
+bool use_rows_dx(int M, int N, int K);
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
                int N, int K, cudaStream_t stream);
 int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,

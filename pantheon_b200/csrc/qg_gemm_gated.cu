@@ -624,21 +624,6 @@ static int check_shape(const char* name, int M, int N, int K) {
 // Terms of dG and dU (see the head of this file).
 static int grad_parts(int M, int N) { return (int64_t)M * N <= 65536 ? 2 : 1; }
 
-// Whether the kernel for few rows takes the forward pass: up to 64 rows, and wherever
-// it splits K four ways or more.  Measured (pairs / few rows, us): 1x1024x1024 8.7 /
-// 3.8, 64x1024x4096 14.1 / 7.9, 64x8192x4096 28.9 / 25.7, 128x8192x4096 (unsplit) 29.9 /
-// 30.5, 128x4096x4096 (four) 20.3 / 17.9, 256x4096x4096 (two) 20.3 / 23.3, 256x1024x1024
-// (four) 10.3 / 7.0, 512x1024x4096 (four) 18.1 / 14.6, 1024x1024x4096 (two) 19.5 / 21.6.
-static bool use_rows(int M, int N, int K) { return M <= 64 || rows_split(M, N, K) >= 4; }
-// And dX, in a launch apart from dWg's and dWu's: more rows only where its contraction
-// is long enough to outweigh that.  All gradients, in one launch / with dX apart:
-// 1x8192x4096 109 / 62 us, 16x8192x4096 78 / 61, 64x1024x4096 25.6 / 18.3, 64x512x512
-// 15.0 / 12.2, 128x1024x512 13.5 / 13.1, 256x4096x1024 31.1 / 25.3, 512x8192x512 45.5 /
-// 36.6; 256x1024x1024 14.5 / 16.2, 512x2048x512 17.8 / 20.5, 1024x512x512 11.4 / 17.6.
-static bool use_rows_dx(int M, int N, int K) {
-    return M <= 64 || (rows_split_dx(M, N, K) >= 4 && M <= 5 * 2 * ceil_div(N, BK));
-}
-
 template <typename T>
 static int forward(const char* name, const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, int act,
                    int M, int N, int K, cudaStream_t stream) {

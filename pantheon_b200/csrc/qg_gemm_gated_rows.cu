@@ -259,8 +259,15 @@ static int make_map(CUtensorMap* map, const void* base, int rows, int cols, int 
                         (uint64_t)cols * 2, BK_BYTES, (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Rows of X per tile.
-static int row_tile(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+// Whether every tile of 64 rows gets four CTAs in one wave (two per SM of 148).
+static bool few_tiles(int M, int tiles_n) { return 4 * (int64_t)tiles_n * ceil_div(M, 64) <= 2 * 148; }
+
+// Rows of X per tile: 128 only where they are many (128 / 64 rows, us: 128x1024x1024 6.5 /
+// 5.3, 256x1024x4096 12.5 / 11.0; 65x4096x4096 16.3 / 19.3, 512x1024x4096 14.4 / 15.8).
+static int row_tile(int M, int tiles_n) {
+    if (M <= 64) return M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    return few_tiles(M, tiles_n) ? 64 : 128;
+}
 
 // x: X, or for dX dG and dU, then their remainders.
 template <typename T, int NT, int ACT, int PARTS>
@@ -286,7 +293,7 @@ static int launch_nt(const void* const (&x)[4], const void* Wg, const void* Wu, 
 template <typename T, int ACT, int PARTS>
 static int launch(const void* const (&x)[4], const void* Wg, const void* Wu, const Params& p, int split,
                   cudaStream_t stream) {
-    switch (row_tile(p.M)) {
+    switch (row_tile(p.M, ceil_div(ACT == DX ? p.K : p.N, ACT == DX ? BW : BW / 2))) {
         case 16: return launch_nt<T, 16, ACT, PARTS>(x, Wg, Wu, p, split, stream);
         case 32: return launch_nt<T, 32, ACT, PARTS>(x, Wg, Wu, p, split, stream);
         case 64: return launch_nt<T, 64, ACT, PARTS>(x, Wg, Wu, p, split, stream);
@@ -297,7 +304,7 @@ static int launch(const void* const (&x)[4], const void* Wg, const void* Wu, con
 // As qg_gemm_mxfp4_rows.cu splits, whose blocks have as many bytes: one wave of two
 // CTAs per SM of 148, four blocks each at least.
 static int pick_split(int M, int tiles_n, int nk) {
-    const int64_t tiles = (int64_t)tiles_n * ceil_div(M, row_tile(M));
+    const int64_t tiles = (int64_t)tiles_n * ceil_div(M, row_tile(M, tiles_n));
     int split = 1;
     while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= nk) split *= 2;
     return split;
@@ -305,15 +312,31 @@ static int pick_split(int M, int tiles_n, int nk) {
 
 } // namespace rows
 
-int rows_split(int M, int N, int K) { return rows::pick_split(M, ceil_div(N, rows::BW / 2), ceil_div(K, rows::BK)); }
+// Forward: up to 64 rows, few tiles, or K split four ways or more.  Measured (pairs / few
+// rows, us): 1x1024x1024 8.7 / 3.8, 64x1024x4096 14.1 / 7.9, 64x8192x4096 28.9 / 25.7,
+// 128x8192x4096 (unsplit) 29.9 / 30.5, 128x4096x4096 (four) 20.3 / 17.9, 256x4096x4096 (two)
+// 20.3 / 23.3, 256x1024x512 7.0 / 6.0, 256x1024x4096 17.8 / 11.0, 512x1024x4096 18.1 / 14.4,
+// 1024x1024x4096 (two) 19.5 / 21.6.
+bool use_rows(int M, int N, int K) {
+    const int tiles_n = ceil_div(N, rows::BW / 2);
+    return M <= 64 || rows::few_tiles(M, tiles_n) || rows::pick_split(M, tiles_n, ceil_div(K, rows::BK)) >= 4;
+}
 
-int rows_split_dx(int M, int N, int K) { return rows::pick_split(M, ceil_div(K, rows::BW), 2 * ceil_div(N, rows::BK)); }
+// dX, in a launch apart from dWg's and dWu's: more rows only where its contraction is
+// long enough to outweigh that.  All gradients, in one launch / with dX apart:
+// 1x8192x4096 109 / 62 us, 16x8192x4096 78 / 61, 64x1024x4096 25.6 / 18.3, 64x512x512
+// 15.0 / 12.2, 128x1024x512 13.5 / 13.1, 256x4096x1024 31.1 / 25.3, 512x8192x512 45.5 /
+// 36.6; 256x1024x1024 14.5 / 16.2, 512x2048x512 17.8 / 20.5, 1024x512x512 11.4 / 17.6.
+bool use_rows_dx(int M, int N, int K) {
+    const int blocks = ceil_div(N, rows::BK);
+    return M <= 64 || (rows::pick_split(M, ceil_div(K, rows::BW), 2 * blocks) >= 4 && M <= 10 * blocks);
+}
 
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
                int N, int K, cudaStream_t stream) {
     const rows::Params p{M, N, K, H, G, U, nullptr};
     const void* const x[4] = {X, nullptr, nullptr, nullptr};
-    const int split = rows_split(M, N, K);
+    const int split = rows::pick_split(M, ceil_div(N, rows::BW / 2), ceil_div(K, rows::BK));
     const bool silu = act == QG_ACT_SILU;
     if (half)
         return silu ? rows::launch<__half, QG_ACT_SILU, 1>(x, Wg, Wu, p, split, stream)
@@ -325,7 +348,7 @@ int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, 
 int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,
                   cudaStream_t stream) {
     const rows::Params p{M, N, K, dX, nullptr, nullptr, nullptr};
-    const int split = rows_split_dx(M, N, K);
+    const int split = rows::pick_split(M, ceil_div(K, rows::BW), 2 * ceil_div(N, rows::BK));
     if (d[2])
         return half ? rows::launch<__half, rows::DX, 2>(d, Wg, Wu, p, split, stream)
                     : rows::launch<__nv_bfloat16, rows::DX, 2>(d, Wg, Wu, p, split, stream);

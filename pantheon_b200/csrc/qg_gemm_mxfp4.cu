@@ -4,7 +4,7 @@
 //   C[m,n] = out( sum_k (qa[m,k] 2^ea[m,k/32]) (qb[n,k] 2^eb[n,k/32]) )
 //   gated: H[m,n] = out( act(A Wg^T)[m,n] * (A Wu^T)[m,n] )
 //
-// Three kernels (use_rows, launch_gemm): few rows or few tiles with a long K
+// Three kernels (use_rows, launch_gemm): few rows or few tiles
 // (qg_gemm_mxfp4_rows.cu), single CTAs for little work, CTA pairs for the rest.  The arithmetic bounds the last: 2 M N K at
 // the fp4 rate; measured 4096x8192x8192 94 us (5.8 PFLOP/s, 0.86 of four times the
 // measured bf16 rate), 8192x8192x16384 341-348 us (6.3-6.4 PFLOP/s, 0.93), tensor pipe
@@ -793,25 +793,13 @@ static int check_mx(const char* name, const void* A, const void* SFA, const void
 
 } // namespace mx
 
-// Whether the kernel for few rows takes it: up to 64 rows (32 of a gated product,
-// whose tiles are half as wide), and wherever it splits K four ways or more, which
-// pays for its own start and join.  Measured, few rows / single / pairs: 64x28672x8192
-// 24.6 / 25.6 / 30.3 us, 128x28672x8192 28.2 / 27.8 / 33.2; 256x1024x8192 (split in
-// eight) 8.8 / 14.9 / 14.2, 256x4096x4096 (four) 9.1 / 9.7 / 9.9, 192x8192x8192 (one)
-// 16.7 / 17.9 / 15.9, 512x4096x14336 (two) 21.4 / - / 22.4, 256x4096x1024 (one) 7.1 /
-// 5.6 / 6.5; gated 64x14336x4096 16.5 / 15.5 / 19.5, 128x14336x4096 19.0 /
-// 16.7 / 20.4.
-static bool use_rows(int M, int N, int K, bool is_gated) {
-    return M <= (is_gated ? 32 : 64) || mx::rows_split(M, N, K, is_gated) >= 4;
-}
-
 int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, void* C, int out_type, int M, int N,
                int K, cudaStream_t stream) {
     int rc = mx::check_mx("qg_gemm_mxfp4", A, SFA, B, SFB, C, M, N, K);
     if (rc) return rc;
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFB), nullptr, C, nullptr,
                      nullptr, 1, false};
-    const bool few = use_rows(M, N, K, false);
+    const bool few = mx::use_rows(M, N, K, false);
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)C % 2 == 0, "qg_gemm_mxfp4: C is not aligned to its element");
@@ -836,7 +824,7 @@ int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void*
     QG_CHECK_ARG(act == QG_ACT_SILU || act == QG_ACT_GELU_TANH, "qg_gemm_gated_mxfp4: unknown activation %d", act);
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFG),
                      static_cast<const uint8_t*>(SFU), H, static_cast<uint8_t*>(SFH), nullptr, 1, false};
-    const bool silu = act == QG_ACT_SILU, few = use_rows(M, N, K, true);
+    const bool silu = act == QG_ACT_SILU, few = mx::use_rows(M, N, K, true);
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)H % 2 == 0, "qg_gemm_gated_mxfp4: H is not aligned to its element");

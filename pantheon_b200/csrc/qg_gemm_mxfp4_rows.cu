@@ -226,11 +226,12 @@ rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUt
                 } else {
                     v[4 * a] = w.x; v[4 * a + 1] = w.y; v[4 * a + 2] = w.z; v[4 * a + 3] = w.w;
                 }
-                // A's tile starts on an atom: m0 is 0, or NT is 128
+                // A's tile is an atom's rows, their first or last 64, or the first few
                 if (NT >= 128) {
                     v[8 + 4 * a] = x.x; v[9 + 4 * a] = x.y; v[10 + 4 * a] = x.z; v[11 + 4 * a] = x.w;
                 } else {
-                    v[8 + 4 * a] = x.x; v[9 + 4 * a] = x.y; v[10 + 4 * a] = 0; v[11 + 4 * a] = 0;
+                    const bool high = m0 & 64;
+                    v[8 + 4 * a] = high ? x.z : x.x; v[9 + 4 * a] = high ? x.w : x.y; v[10 + 4 * a] = 0; v[11 + 4 * a] = 0;
                 }
             }
             __syncwarp();
@@ -375,12 +376,34 @@ static int launch_nt(const void* X, const void* W, const void* W2, Params p, int
     return QG_OK;
 }
 
-// Rows of A per tile.
-static int row_tile(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+// Whether every tile of 64 rows gets four CTAs in one wave (two per SM of 148).
+static bool few_tiles(int M, int tiles_n) { return 4 * (int64_t)tiles_n * ceil_div(M, 64) <= 2 * 148; }
+
+// Rows of A per tile: 128 only where they are many (128 / 64 rows, us: 128x1024x4096
+// 6.4 / 5.3, 512x1024x8192 10.5 / 8.4, 512x1024x4096 6.8 / 6.9).
+static int row_tile(int M, int tiles_n) {
+    if (M <= 64) return M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    return few_tiles(M, tiles_n) ? 64 : 128;
+}
+
+// CTAs that share a tile's K.
+static int pick_split(int M, int tiles_n, int K) {
+    const int nk = (K + BK - 1) / BK;
+    const int64_t tiles = (int64_t)tiles_n * ceil_div(M, row_tile(M, tiles_n));
+    // As many CTAs as one wave holds, four K blocks each at least: a CTA's start and
+    // end cost 2-3 us, which a second wave pays again, and the join grows with the
+    // split.  Measured (one row, K=8192): N=28672 22.8 us unsplit, 26.1 in two, 31.5 in
+    // four; N=8192 14.1, 10.7, 10.4 and 13.9 in eight; N=1024 13.3, 8.6, 6.2, 5.1.
+    // 333 x 1001 x 4128 (17 blocks): 7.4 in four, 9.6 in eight.
+    int split = 1;
+    while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= nk) split *= 2;
+    return split;
+}
 
 template <int OUT, int ACT>
 static int launch(const void* X, const void* W, const void* W2, const Params& p, cudaStream_t stream) {
-    const int nt = row_tile(p.M), split = rows_split(p.M, p.N, p.K, ACT >= 0);
+    const int tiles_n = ceil_div(p.N, ACT >= 0 ? BW / 2 : BW);
+    const int nt = row_tile(p.M, tiles_n), split = pick_split(p.M, tiles_n, p.K);
     switch (nt) {
         case 16: return launch_nt<16, OUT, ACT>(X, W, W2, p, split, stream);
         case 32: return launch_nt<32, OUT, ACT>(X, W, W2, p, split, stream);
@@ -391,18 +414,17 @@ static int launch(const void* X, const void* W, const void* W2, const Params& p,
 
 } // namespace rows
 
-int rows_split(int M, int N, int K, bool is_gated) {
-    using namespace rows;
-    const int nk = (K + BK - 1) / BK;
-    const int64_t tiles = (int64_t)ceil_div(N, is_gated ? BW / 2 : BW) * ceil_div(M, row_tile(M));
-    // As many CTAs as one wave holds (two per SM of 148), four K blocks each at least:
-    // a CTA's start and end cost 2-3 us, which a second wave pays again, and the join
-    // grows with the split.  Measured (one row, K=8192): N=28672 22.8 us unsplit, 26.1
-    // in two, 31.5 in four; N=8192 14.1, 10.7, 10.4 and 13.9 in eight; N=1024 13.3, 8.6,
-    // 6.2, 5.1.  333 x 1001 x 4128 (17 blocks): 7.4 in four, 9.6 in eight.
-    int split = 1;
-    while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= nk) split *= 2;
-    return split;
+// Up to 64 rows (32 of a gated product, whose tiles are half as wide), few tiles, or
+// K split four ways or more, which pays for its own start and join.  Measured, few
+// rows / single / pairs: 64x28672x8192 24.6 / 25.6 / 30.3 us, 128x28672x8192 28.2 / 27.8 /
+// 33.2; 256x1024x512 4.5 / 4.8 / -, 512x1024x2048 6.1 / 7.0 / -, 128x4096x4096 6.9 / 6.8
+// (few tiles); 256x1024x8192 8.8 / 14.9 / 14.2, 256x4096x4096 9.1 / 9.7 / 9.9 (split in
+// eight, four); 192x8192x8192 16.7 / 17.9 / 15.9, 512x4096x14336 21.4 / - / 22.4,
+// 256x4096x1024 7.1 / 5.6 / 6.5 (neither); gated 64x14336x4096 16.5 / 15.5 / 19.5,
+// 128x14336x4096 19.0 / 16.7 / 20.4.
+bool use_rows(int M, int N, int K, bool is_gated) {
+    const int tiles_n = ceil_div(N, is_gated ? rows::BW / 2 : rows::BW);
+    return M <= (is_gated ? 32 : 64) || rows::few_tiles(M, tiles_n) || rows::pick_split(M, tiles_n, K) >= 4;
 }
 
 int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,

@@ -142,7 +142,8 @@ def test_gated_matches_the_definition(cuda_device, shape, act):
 # several, CTA pairs (more than 148 tiles, or K over 4096) with their last row tile in the first or
 # the second CTA and with several tiles each, and the kernel for few rows with K split on many rows
 WIDE = [(70, 19001, 288), (130, 10001, 544), (200, 5024, 1056), (513, 9999, 96), (1400, 4320, 800), (130, 9999, 4128),
-        (300, 1001, 4128), (130, 257, 8224), (200, 5026, 1056), (520, 5004, 96), (1300, 2050, 224)]
+        (300, 1001, 4128), (130, 257, 8224), (200, 5026, 1056), (520, 5004, 96), (1300, 2050, 224),
+        (200, 3091, 4128)]
 
 
 @pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32])
@@ -155,6 +156,23 @@ def test_wide_gemm_matches_the_definition(cuda_device, shape, out_type):
     y = _np(pb.gemm_mxfp4(*a, *b, out_type=out_type))
     assert (np.abs(y - ref) <= e + (2.0 ** -8 * np.abs(ref) if out_type == pb.QG_OUT_BF16 else 0)).all()
     assert pb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("offset", [1, 2, 4])
+@pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32])
+@pytest.mark.parametrize("shape", [(3, 264, 128), (130, 10000, 128), (130, 10001, 128), (520, 5000, 128), (520, 5001, 128)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gemm_into_a_tensor_off_16_bytes(cuda_device, shape, out_type, offset):
+    """Rows at every place, the elements before and behind the result left as they were."""
+    M, N, K = shape
+    a, _ = _operand(M, K, M + K, cuda_device)
+    b, _ = _operand(N, K, N + 3 * K, cuda_device)
+    ref = pb.gemm_mxfp4(*a, *b, out_type=out_type)
+    flat = torch.full((offset + M * N + 8,), -7.0, dtype=ref.dtype, device=cuda_device)
+    out = flat[offset:offset + M * N].view(M, N)
+    assert pb.gemm_mxfp4(*a, *b, out_type=out_type, out=out) is out
+    assert torch.equal(out, ref)
+    assert (flat[:offset] == -7).all() and (flat[offset + M * N:] == -7).all()
 
 
 @pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32, pb.QG_OUT_MXFP4])
