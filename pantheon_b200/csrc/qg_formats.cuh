@@ -85,10 +85,11 @@ int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, co
 }
 namespace ffn {
 // The forward pass and dX of the gated block of 16-bit operands for few rows of X
-// (qg_gemm_gated_rows.cu): whether that kernel takes them, and its launches.  G and U
-// null or kept; d = dG, dU and their remainders (null: none).
+// (qg_gemm_gated_rows.cu): whether that kernel takes the forward pass, among how many
+// CTAs it splits a tile of dX, and the launches.  G and U null or kept; d = dG, dU and
+// their remainders (null: none).
 bool use_rows(int M, int N, int K);
-bool use_rows_dx(int M, int N, int K);
+int rows_split_dx(int M, int N, int K);
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
                int N, int K, cudaStream_t stream);
 int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,

@@ -647,18 +647,32 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
                               : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
 }
 
-// The products of the backward pass (dx_apart: dWg and dWu).
-template <typename T, int PARTS>
-static int products(const Maps& maps, bool dx_apart, void* dX, void* dWg, void* dWu, int M, int N, int K,
+// Whether dX goes to the kernel for few rows, in a launch apart from dWg's and dWu's:
+// more rows only where its contraction is long enough to outweigh that, or where dX
+// would have a launch of its own anyway.  All gradients, in one launch / with dX apart:
+// 1x8192x4096 109 / 62 us, 16x8192x4096 78 / 61, 64x1024x4096 25.6 / 18.3, 64x512x512
+// 15.0 / 12.2, 128x1024x512 13.5 / 13.1, 256x4096x1024 31.1 / 25.3, 512x8192x512 45.5 /
+// 36.6; 256x1024x1024 14.5 / 16.2, 512x2048x512 17.8 / 20.5, 1024x512x512 11.4 / 17.6.
+// In two launches of the pairs / with dX here: 256x1024x2048 21.6 / 16.7,
+// 384x2048x1024 25.0 / 19.9, 768x4096x512 34.3 / 28.8.
+static bool use_rows_dx(int M, int N, int K, bool apart_anyway) {
+    return M <= 64 || (rows_split_dx(M, N, K) >= 4 && (apart_anyway || M <= 10 * ceil_div(N, BK)));
+}
+
+// The products of the backward pass; rows_dx() launches dX by the kernel for few rows.
+template <typename T, int PARTS, typename F>
+static int products(const Maps& maps, const F& rows_dx, void* dX, void* dWg, void* dWu, int M, int N, int K,
                     const DeviceInfo* info, cudaStream_t stream) {
     int rc;
     const int nk_dx = 2 * ceil_div(N, BK), nk_dw = ceil_div(M, BK);
     const int64_t units_dx = (int64_t)ceil_div(M, 2 * BM) * ceil_div(K, BN);
     const int64_t units_dw = 2 * (int64_t)ceil_div(N, 2 * BM) * ceil_div(K, BN);
-    if (dx_apart) {
+    auto dx_apart = [&] {
         const Params p{M, N, K, 0, 1, 0, 0, 1, 1, 0, 1, nullptr, dWg, dWu, nullptr};
-        return launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units_dw, nk_dw, stream);
-    }
+        if (dX && (rc = rows_dx())) return rc;
+        return dWg ? launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units_dw, nk_dw, stream) : QG_OK;
+    };
+    if (use_rows_dx(M, N, K, false)) return dx_apart();
     // One launch for the three: all tiles split; or the long ones, where they are few of
     // many blocks beside many of few (dX with few rows of X, dWg and dWu with many) and
     // all fit at once; or none split.  Where the long ones should be split and do not
@@ -685,6 +699,7 @@ static int products(const Maps& maps, bool dx_apart, void* dX, void* dWg, void* 
             if ((rc = device_status_ptr(&q.status))) return rc;
             return launch_kernel<T, true, QG_ACT_SILU, true, PARTS>(maps, q, beside, info, stream);
         }
+        if (!dw_first && use_rows_dx(M, N, K, true)) return dx_apart();
         (dw_first ? q.tiles_dx : q.tiles_dw) = 0;
         if ((dw_first ? dWg : dX) && (rc = launch<T, true, QG_ACT_SILU, PARTS>(maps, q, units, nk, stream))) return rc;
         q = p;
@@ -724,28 +739,27 @@ static int backward(const char* name, const void* dH, const void* X, const void*
                              : (silu ? gate_backward_kernel<T, QG_ACT_SILU, 1> : gate_backward_kernel<T, QG_ACT_GELU_TANH, 1>);
     QG_CUDA(launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, 1, vh, vg, vu,
                               static_cast<uint4*>(workspace), n8));
-    const bool dx_apart = use_rows_dx(M, N, K);
-    if (dx_apart && dX) {
+    auto rows_dx = [&] {
         const void* d[4] = {};
         for (int i = 0; i < 2 * parts; ++i) d[i] = static_cast<const uint8_t*>(workspace) + i * one;
-        if ((rc = gated_rows_dx(d, Wg, Wu, dX, std::is_same<T, __half>::value, M, N, K, stream))) return rc;
-    }
-    if (dx_apart && !dWg) return QG_OK;
+        return gated_rows_dx(d, Wg, Wu, dX, std::is_same<T, __half>::value, M, N, K, stream);
+    };
+    const bool no_dx = use_rows_dx(M, N, K, false);             // (its operands' maps are not read)
     Maps maps;
     if ((rc = make_map(&maps.x, X, M, K, BK))) return rc;
     for (int w = 0; w < 2; ++w)
         for (int q = 0; q < 2; ++q) {
             void* d = static_cast<uint8_t*>(workspace) + (2 * q + w) * one;
-            // (the second terms of one, and dX's operands where it is apart, are not read)
+            // (the second term of one is not read)
             if (q >= parts) maps.cols[w][q] = maps.cols[w][0];
             else if ((rc = make_map(&maps.cols[w][q], d, M, N, BK))) return rc;
-            if (q >= parts || dx_apart) maps.rows[w][q] = maps.cols[w][q];
+            if (q >= parts || no_dx) maps.rows[w][q] = maps.cols[w][q];
             else if ((rc = make_map(&maps.rows[w][q], d, M, N, BM))) return rc;
         }
     maps.wg = maps.wu = maps.x;
-    if (!dx_apart && ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)))) return rc;
-    return parts == 2 ? products<T, 2>(maps, dx_apart, dX, dWg, dWu, M, N, K, info, stream)
-                      : products<T, 1>(maps, dx_apart, dX, dWg, dWu, M, N, K, info, stream);
+    if (!no_dx && ((rc = make_map(&maps.wg, Wg, N, K, BK)) || (rc = make_map(&maps.wu, Wu, N, K, BK)))) return rc;
+    return parts == 2 ? products<T, 2>(maps, rows_dx, dX, dWg, dWu, M, N, K, info, stream)
+                      : products<T, 1>(maps, rows_dx, dX, dWg, dWu, M, N, K, info, stream);
 }
 
 } // namespace ffn

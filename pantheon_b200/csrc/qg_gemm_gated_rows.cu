@@ -322,15 +322,7 @@ bool use_rows(int M, int N, int K) {
     return M <= 64 || rows::few_tiles(M, tiles_n) || rows::pick_split(M, tiles_n, ceil_div(K, rows::BK)) >= 4;
 }
 
-// dX, in a launch apart from dWg's and dWu's: more rows only where its contraction is
-// long enough to outweigh that.  All gradients, in one launch / with dX apart:
-// 1x8192x4096 109 / 62 us, 16x8192x4096 78 / 61, 64x1024x4096 25.6 / 18.3, 64x512x512
-// 15.0 / 12.2, 128x1024x512 13.5 / 13.1, 256x4096x1024 31.1 / 25.3, 512x8192x512 45.5 /
-// 36.6; 256x1024x1024 14.5 / 16.2, 512x2048x512 17.8 / 20.5, 1024x512x512 11.4 / 17.6.
-bool use_rows_dx(int M, int N, int K) {
-    const int blocks = ceil_div(N, rows::BK);
-    return M <= 64 || (rows::pick_split(M, ceil_div(K, rows::BW), 2 * blocks) >= 4 && M <= 10 * blocks);
-}
+int rows_split_dx(int M, int N, int K) { return rows::pick_split(M, ceil_div(K, rows::BW), 2 * ceil_div(N, rows::BK)); }
 
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
                int N, int K, cudaStream_t stream) {
@@ -348,7 +340,7 @@ int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, 
 int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,
                   cudaStream_t stream) {
     const rows::Params p{M, N, K, dX, nullptr, nullptr, nullptr};
-    const int split = rows::pick_split(M, ceil_div(K, rows::BW), 2 * ceil_div(N, rows::BK));
+    const int split = rows_split_dx(M, N, K);
     if (d[2])
         return half ? rows::launch<__half, rows::DX, 2>(d, Wg, Wu, p, split, stream)
                     : rows::launch<__nv_bfloat16, rows::DX, 2>(d, Wg, Wu, p, split, stream);

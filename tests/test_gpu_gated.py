@@ -103,7 +103,7 @@ def test_forward_of_few_rows(cuda_device, shape, kind):
 FEW_DX = [(1, 8, 8), (1, 4104, 136), (7, 9608, 264), (16, 520, 1000), (20, 1032, 136), (40, 3000, 72), (64, 264, 9608),
           (65, 1032, 264), (100, 2056, 1000), (129, 4104, 136), (130, 264, 72), (1300, 520, 264), (2050, 520, 520),
           (32, 4104, 72), (40, 1032, 136), (66, 520, 136), (300, 4104, 264),
-          (200, 1288, 3104), (100, 600, 5000)]
+          (200, 1288, 3104), (100, 600, 5000), (270, 800, 1800)]
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
