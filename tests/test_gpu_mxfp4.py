@@ -177,7 +177,8 @@ def test_gemm_into_a_tensor_off_16_bytes(cuda_device, shape, out_type, offset):
 
 @pytest.mark.parametrize("out_type", [pb.QG_OUT_BF16, pb.QG_OUT_F32, pb.QG_OUT_MXFP4])
 @pytest.mark.parametrize("shape", [(40, 9601, 288), (64, 9632, 352), (130, 5001, 544), (200, 4928, 1056), (513, 5024, 96),
-                                   (1400, 2176, 416), (200, 4928, 4128), (300, 480, 4128), (200, 5026, 96), (1400, 2179, 416)], ids=lambda s: "x".join(map(str, s)))
+                                   (1400, 2176, 416), (200, 4928, 4128), (300, 480, 4128), (200, 5026, 96), (1400, 2179, 416), (100, 96, 512),
+                                   (190, 165, 2048)], ids=lambda s: "x".join(map(str, s)))
 def test_wide_gated_matches_the_definition(cuda_device, shape, out_type):
     M, N, K = shape
     if out_type == pb.QG_OUT_MXFP4 and N % 32:
