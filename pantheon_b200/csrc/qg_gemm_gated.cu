@@ -486,12 +486,12 @@ gated_kernel(const __grid_constant__ Maps maps, const Params p) {
 // 2 bytes per element: bound by memory (4096x8192 in 47 us, 7.1 TB/s).
 template <typename T, int ACT, int PARTS>
 __global__ void __launch_bounds__(256)
-gate_backward_kernel(const uint4* __restrict__ dH, const uint4* __restrict__ G, const uint4* __restrict__ U,
-                     uint4* __restrict__ D, uint64_t n8) {
+gate_backward_kernel(const uint4* dH, const uint4* G, const uint4* U,
+                     uint4* D, uint64_t n8) {
     wait_previous_grid();
     const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n8) return;
-    const uint4 vh = __ldg(dH + i), vg = __ldg(G + i), vu = __ldg(U + i);
+    const uint4 vh = load_global(dH + i), vg = load_global(G + i), vu = load_global(U + i);
     const uint32_t h[4] = {vh.x, vh.y, vh.z, vh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
     uint32_t o[2][2][4];
 #pragma unroll

@@ -54,7 +54,7 @@ __device__ __forceinline__ void load(const T* src, int n, uintptr_t begin, uintp
     if (whole) {
 #pragma unroll
         for (int i = 0; i < (VEC ? 2 : 3); ++i) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(base) + i);
+            const uint4 q = load_global(reinterpret_cast<const uint4*>(base) + i);
             v.w[4 * i] = q.x; v.w[4 * i + 1] = q.y; v.w[4 * i + 2] = q.z; v.w[4 * i + 3] = q.w;
         }
         return;
@@ -67,12 +67,12 @@ __device__ __forceinline__ void load(const T* src, int n, uintptr_t begin, uintp
     for (int i = 0; i < (VEC ? 8 : 12); ++i) {
         if constexpr (sizeof(T) == 4) {
             const int j = i - off / 4;
-            if (j >= 0 && j < n) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + j);
+            if (j >= 0 && j < n) v.w[i] = load_global(reinterpret_cast<const uint32_t*>(src) + j);
         } else {
             const int j = 2 * i - off / 2;
             const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-            if (j >= 0 && j < n) v.w[i] = __ldg(h + j);
-            if (j + 1 >= 0 && j + 1 < n) v.w[i] |= (uint32_t)__ldg(h + j + 1) << 16;
+            if (j >= 0 && j < n) v.w[i] = load_global(h + j);
+            if (j + 1 >= 0 && j + 1 < n) v.w[i] |= load_global(h + j + 1) << 16;
         }
     }
 }
@@ -134,7 +134,7 @@ __device__ __forceinline__ float value(const Raw<T>& v, int i) {
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS)
-quant_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q, uint8_t* __restrict__ SF, int M, int K) {
+quant_kernel(const T* X, int64_t ldx, uint8_t* Q, uint8_t* SF, int M, int K) {
     constexpr int N = Raw<T>::N;                              // 16 or 8 values, 2 or 4 lanes per block
     const int lane = threadIdx.x & 31;
     const int kp = (K + BLOCK - 1) / BLOCK * BLOCK;          // columns that have codes
@@ -199,7 +199,7 @@ __device__ __forceinline__ float2 unpack2(uint32_t byte) {
 // The reverse, in the same shape: a lane's four bytes of a row are eight values.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
-dequant_kernel(const uint8_t* __restrict__ Q, const uint8_t* __restrict__ SF, T* __restrict__ Y, int M, int K) {
+dequant_kernel(const uint8_t* Q, const uint8_t* SF, T* Y, int M, int K) {
     const int lane = threadIdx.x & 31;
     const int kchunks = (K + ATOM_K - 1) / ATOM_K;
     const int segs = (K + SEG - 1) / SEG;
@@ -215,8 +215,8 @@ dequant_kernel(const uint8_t* __restrict__ Q, const uint8_t* __restrict__ SF, T*
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int r = r0 + i < M ? r0 + i : M - 1;
-        w[i] = __ldg(reinterpret_cast<const uint32_t*>(Q + (size_t)r * (K / 2) + k0 / 2));
-        s[i] = __ldg(SF + sf_offset(r, k0 / BLOCK, kchunks));
+        w[i] = load_global(reinterpret_cast<const uint32_t*>(Q + (size_t)r * (K / 2) + k0 / 2));
+        s[i] = load_global(SF + sf_offset(r, k0 / BLOCK, kchunks));
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
