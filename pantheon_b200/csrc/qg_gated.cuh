@@ -37,12 +37,16 @@ __device__ __forceinline__ float gated(float g, float u) {
     return g * logistic<FAST>(gate_arg<ACT>(g)) * u;
 }
 
-// act(g) and its slope.  p (1 - p) is 0 in fp32 from |g| = 30 on, where g^2
-// must not overflow against it: the bend's argument is cut off there.
+// act(g) and its slope.  An infinite or huge g must not meet 1 - p = 0 (or p = 0) in
+// a product, so the bend's argument is cut off where its factor p (1 - p) is exactly
+// 0 in fp32 on either side: for silu beyond |g| = 87.4, where p is cut off (at -30 p
+// is still 9.4e-14 and the slope -29 p); for gelu, whose logistic has 2 sqrt(2/pi)
+// (1 + 0.044715 g^2) g for its argument (-1974 at -30), beyond 30, before g^2 grows.
 template <int ACT>
 __device__ __forceinline__ void gate_slope(float g, float& a, float& s) {
+    constexpr float CUT = ACT == QG_ACT_SILU ? 100.0f : 30.0f;
     const float p = logistic<true>(gate_arg<ACT>(g));
-    const float c = fminf(fmaxf(g, -30.0f), 30.0f);
+    const float c = fminf(fmaxf(g, -CUT), CUT);
     const float dy = ACT == QG_ACT_SILU ? 1.0f : fmaf(3.0f * 0.0713548162726f, c * c, 1.59576912161f);
     a = g * p;
     s = fmaf(c * p * (1.0f - p), dy, p);
