@@ -277,7 +277,7 @@ static int launch_quant(const void* X, int64_t ldx, void* Q, void* SF, int M, in
 } // namespace mx
 
 uint64_t mxfp4_sf_bytes(int rows, int K) {
-    return (uint64_t)((rows + 127) / 128) * (uint64_t)((K + mx::ATOM_K - 1) / mx::ATOM_K) * mx::ATOM_BYTES;
+    return ((uint64_t)rows + 127) / 128 * (((uint64_t)K + mx::ATOM_K - 1) / mx::ATOM_K) * mx::ATOM_BYTES;
 }
 
 int quant_mxfp4(const void* X, int in_type, int64_t ldx, void* Q, void* SF, int M, int K, cudaStream_t s) {
@@ -301,6 +301,7 @@ int dequant_mxfp4(const void* Q, const void* SF, void* Y, int out_type, int M, i
     QG_CHECK_ARG(Q && SF && Y, "qg_dequant_mxfp4: null operand or output");
     QG_CHECK_ARG(M > 0 && K > 0, "qg_dequant_mxfp4: empty shape %dx%d", M, K);
     QG_CHECK_ARG(K % 32 == 0, "qg_dequant_mxfp4: K=%d must be a multiple of 32", K);
+    QG_CHECK_ARG(M <= INT32_MAX - 127 && K <= INT32_MAX - 511, "qg_dequant_mxfp4: shape %dx%d is too large", M, K);
     QG_CHECK_ARG(((uintptr_t)Q & 15) == 0 && ((uintptr_t)SF & 15) == 0 && ((uintptr_t)Y & 15) == 0,
                  "qg_dequant_mxfp4: codes, scales and output must be 16-byte aligned");
     QG_CHECK_ARG(out_type == QG_OUT_BF16 || out_type == QG_OUT_F32, "qg_dequant_mxfp4: out_type %d (bf16 or f32)",
