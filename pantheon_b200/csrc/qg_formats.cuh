@@ -77,23 +77,23 @@ int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, v
 int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void* SFG, const void* Wu, const void* SFU,
                      void* H, void* SFH, int out_type, int act, int M, int N, int K, cudaStream_t stream);
 namespace mx {
-// Whether the kernel for few rows takes a product (qg_gemm_mxfp4_rows.cu), and its launch; act < 0
-// is the plain one.  Arguments are checked by the caller.
-bool use_rows(int M, int N, int K, bool is_gated);
+// Whether the kernel for few rows takes a product (qg_gemm_mxfp4_rows.cu) on a device of `sms`
+// SMs, and its launch; act < 0 is the plain one.  Arguments are checked by the caller.
+bool use_rows(int M, int N, int K, bool is_gated, int sms);
 int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,
-              void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream);
+              void* SFC, int out_type, int act, bool vec, int M, int N, int K, int sms, cudaStream_t stream);
 }
 namespace ffn {
 // The forward pass and dX of the gated block of 16-bit operands for few rows of X
 // (qg_gemm_gated_rows.cu): whether that kernel takes the forward pass, among how many
 // CTAs it splits a tile of dX, and the launches.  G and U null or kept; d = dG, dU and
 // their remainders (null: none).
-bool use_rows(int M, int N, int K);
-int rows_split_dx(int M, int N, int K);
+bool use_rows(int M, int N, int K, int sms);
+int rows_split_dx(int M, int N, int K, int sms);
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
-               int N, int K, cudaStream_t stream);
+               int N, int K, int sms, cudaStream_t stream);
 int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,
-                  cudaStream_t stream);
+                  int sms, cudaStream_t stream);
 }
 int gen_w4a16(void* X, void* W, void* S, void* Z, int M, int N, int K, uint64_t seed, uint32_t tid0, cudaStream_t s);
 uint64_t gemv_w4a16_workspace_bytes(int M, int N, int K, int sm_count);

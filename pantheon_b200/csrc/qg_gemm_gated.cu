@@ -58,6 +58,7 @@ namespace ffn {
 
 using mx::elect_one;
 using mx::mbar_arrive_relaxed;
+using mx::umma_commit_both;
 using mx::warp_wait;
 
 enum : int { FWD = 0, DX = 1, DW = 2 };
@@ -199,12 +200,6 @@ __device__ __forceinline__ void load_operand(uint8_t* dst, const CUtensorMap* ma
     } else {
         tma_load_2d_pair(dst, map, bar, k0 * 2, row0);
     }
-}
-
-// One commit that arrives on the same barrier of both CTAs of a pair.
-__device__ __forceinline__ void umma_commit_both(uint64_t* bar, uint32_t pair_in_cluster) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_u32(bar)), "h"((uint16_t)(3u << (2 * pair_in_cluster))) : "memory");
 }
 
 template <typename T>
@@ -600,10 +595,8 @@ static int pick_split(int* out, int64_t units, int nk, const DeviceInfo* info) {
 }
 
 template <typename T, bool BACK, int ACT, int PARTS = 1>
-static int launch(const Maps& maps, Params p, int64_t units, int nk, cudaStream_t stream) {
-    DeviceInfo* info = nullptr;
-    int rc = current_device_info(&info);
-    if (rc) return rc;
+static int launch(const Maps& maps, Params p, int64_t units, int nk, const DeviceInfo* info, cudaStream_t stream) {
+    int rc;
     if ((rc = device_status_ptr(&p.status))) return rc;
     int subs = 1;
     if ((rc = pick_split<T, BACK, ACT>(&subs, units, nk, info))) return rc;
@@ -634,7 +627,10 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
     if (rc) return rc;
     QG_CHECK_ARG((((uintptr_t)X | (uintptr_t)Wg | (uintptr_t)Wu | (uintptr_t)H | (uintptr_t)G | (uintptr_t)U) & 15) == 0,
                  "%s: operands and outputs must be 16-byte aligned", name);
-    if (use_rows(M, N, K)) return gated_rows(X, Wg, Wu, H, G, U, std::is_same<T, __half>::value, act, M, N, K, stream);
+    DeviceInfo* info = nullptr;
+    if ((rc = current_device_info(&info))) return rc;
+    if (use_rows(M, N, K, info->sm_count))
+        return gated_rows(X, Wg, Wu, H, G, U, std::is_same<T, __half>::value, act, M, N, K, info->sm_count, stream);
     Maps maps;
     if ((rc = make_map(&maps.x, X, M, K, BM)) || (rc = make_map(&maps.wg, Wg, N, K, 128)) ||
         (rc = make_map(&maps.wu, Wu, N, K, 128)))
@@ -643,8 +639,8 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
     const uint64_t group = GROUP_X_BYTES / ((uint64_t)2 * BM * (uint64_t)K * 2);
     const Params p{M, N, K, 0, 0, 0, 0, 0, 0, 0, (int)(group < 1 ? 1 : group > 64 ? 64 : group), H, G, U, nullptr};
     const int64_t units = (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN / 2);
-    return act == QG_ACT_SILU ? launch<T, false, QG_ACT_SILU>(maps, p, units, ceil_div(K, BK), stream)
-                              : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), stream);
+    return act == QG_ACT_SILU ? launch<T, false, QG_ACT_SILU>(maps, p, units, ceil_div(K, BK), info, stream)
+                              : launch<T, false, QG_ACT_GELU_TANH>(maps, p, units, ceil_div(K, BK), info, stream);
 }
 
 // Whether dX goes to the kernel for few rows, in a launch apart from dWg's and dWu's:
@@ -655,8 +651,8 @@ static int forward(const char* name, const void* X, const void* Wg, const void* 
 // 36.6; 256x1024x1024 14.5 / 16.2, 512x2048x512 17.8 / 20.5, 1024x512x512 11.4 / 17.6.
 // In two launches of the pairs / with dX here: 256x1024x2048 21.6 / 16.7,
 // 384x2048x1024 25.0 / 19.9, 768x4096x512 34.3 / 28.8.
-static bool use_rows_dx(int M, int N, int K, bool apart_anyway) {
-    return M <= 64 || (rows_split_dx(M, N, K) >= 4 && (apart_anyway || M <= 10 * ceil_div(N, BK)));
+static bool use_rows_dx(int M, int N, int K, bool apart_anyway, int sms) {
+    return M <= 64 || (rows_split_dx(M, N, K, sms) >= 4 && (apart_anyway || M <= 10 * ceil_div(N, BK)));
 }
 
 // The products of the backward pass; rows_dx() launches dX by the kernel for few rows.
@@ -670,9 +666,9 @@ static int products(const Maps& maps, const F& rows_dx, void* dX, void* dWg, voi
     auto dx_apart = [&] {
         const Params p{M, N, K, 0, 1, 0, 0, 1, 1, 0, 1, nullptr, dWg, dWu, nullptr};
         if (dX && (rc = rows_dx())) return rc;
-        return dWg ? launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units_dw, nk_dw, stream) : QG_OK;
+        return dWg ? launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units_dw, nk_dw, info, stream) : QG_OK;
     };
-    if (use_rows_dx(M, N, K, false)) return dx_apart();
+    if (use_rows_dx(M, N, K, false, info->sm_count)) return dx_apart();
     // One launch for the three: all tiles split; or the long ones, where they are few of
     // many blocks beside many of few (dX with few rows of X, dWg and dWu with many) and
     // all fit at once; or none split.  Where the long ones should be split and do not
@@ -699,15 +695,15 @@ static int products(const Maps& maps, const F& rows_dx, void* dX, void* dWg, voi
             if ((rc = device_status_ptr(&q.status))) return rc;
             return launch_kernel<T, true, QG_ACT_SILU, true, PARTS>(maps, q, beside, info, stream);
         }
-        if (!dw_first && use_rows_dx(M, N, K, true)) return dx_apart();
+        if (!dw_first && use_rows_dx(M, N, K, true, info->sm_count)) return dx_apart();
         (dw_first ? q.tiles_dx : q.tiles_dw) = 0;
-        if ((dw_first ? dWg : dX) && (rc = launch<T, true, QG_ACT_SILU, PARTS>(maps, q, units, nk, stream))) return rc;
+        if ((dw_first ? dWg : dX) && (rc = launch<T, true, QG_ACT_SILU, PARTS>(maps, q, units, nk, info, stream))) return rc;
         q = p;
         (dw_first ? q.tiles_dw : q.tiles_dx) = 0;
-        if ((dw_first ? dX : dWg) && (rc = launch<T, true, QG_ACT_SILU, PARTS>(maps, q, units_short, nk_short, stream))) return rc;
+        if ((dw_first ? dX : dWg) && (rc = launch<T, true, QG_ACT_SILU, PARTS>(maps, q, units_short, nk_short, info, stream))) return rc;
         return QG_OK;
     }
-    return launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units + units_short, nk, stream);
+    return launch<T, true, QG_ACT_SILU, PARTS>(maps, p, units + units_short, nk, info, stream);
 }
 
 template <typename T>
@@ -742,9 +738,9 @@ static int backward(const char* name, const void* dH, const void* X, const void*
     auto rows_dx = [&] {
         const void* d[4] = {};
         for (int i = 0; i < 2 * parts; ++i) d[i] = static_cast<const uint8_t*>(workspace) + i * one;
-        return gated_rows_dx(d, Wg, Wu, dX, std::is_same<T, __half>::value, M, N, K, stream);
+        return gated_rows_dx(d, Wg, Wu, dX, std::is_same<T, __half>::value, M, N, K, info->sm_count, stream);
     };
-    const bool no_dx = use_rows_dx(M, N, K, false);             // (its operands' maps are not read)
+    const bool no_dx = use_rows_dx(M, N, K, false, info->sm_count);             // (its operands' maps are not read)
     Maps maps;
     if ((rc = make_map(&maps.x, X, M, K, BK))) return rc;
     for (int w = 0; w < 2; ++w)

@@ -25,6 +25,7 @@
 //   warps 2-5   epilogue.
 // All barrier waits are bounded (qg_ptx.cuh).
 #include "qg_common.cuh"
+#include "qg_few_rows.cuh"
 #include "qg_formats.cuh"
 #include "qg_gated.cuh"
 #include "qg_launch.cuh"
@@ -259,16 +260,6 @@ static int make_map(CUtensorMap* map, const void* base, int rows, int cols, int 
                         (uint64_t)cols * 2, BK_BYTES, (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Whether every tile of 64 rows gets four CTAs in one wave (two per SM of 148).
-static bool few_tiles(int M, int tiles_n) { return 4 * (int64_t)tiles_n * ceil_div(M, 64) <= 2 * 148; }
-
-// Rows of X per tile: 128 only where they are many (128 / 64 rows, us: 128x1024x1024 6.5 /
-// 5.3, 256x1024x4096 12.5 / 11.0; 65x4096x4096 16.3 / 19.3, 512x1024x4096 14.4 / 15.8).
-static int row_tile(int M, int tiles_n) {
-    if (M <= 64) return M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    return few_tiles(M, tiles_n) ? 64 : 128;
-}
-
 // x: X, or for dX dG and dU, then their remainders.
 template <typename T, int NT, int ACT, int PARTS>
 static int launch_nt(const void* const (&x)[4], const void* Wg, const void* Wu, Params p, int split, cudaStream_t stream) {
@@ -291,23 +282,16 @@ static int launch_nt(const void* const (&x)[4], const void* Wg, const void* Wu, 
 }
 
 template <typename T, int ACT, int PARTS>
-static int launch(const void* const (&x)[4], const void* Wg, const void* Wu, const Params& p, int split,
+static int launch(const void* const (&x)[4], const void* Wg, const void* Wu, const Params& p, int sms,
                   cudaStream_t stream) {
-    switch (row_tile(p.M, ceil_div(ACT == DX ? p.K : p.N, ACT == DX ? BW : BW / 2))) {
+    const int tiles_n = ACT == DX ? ceil_div(p.K, BW) : ceil_div(p.N, BW / 2);
+    const int split = few_rows::pick_split(p.M, tiles_n, ACT == DX ? 2 * ceil_div(p.N, BK) : ceil_div(p.K, BK), sms);
+    switch (few_rows::row_tile(p.M, tiles_n, sms)) {
         case 16: return launch_nt<T, 16, ACT, PARTS>(x, Wg, Wu, p, split, stream);
         case 32: return launch_nt<T, 32, ACT, PARTS>(x, Wg, Wu, p, split, stream);
         case 64: return launch_nt<T, 64, ACT, PARTS>(x, Wg, Wu, p, split, stream);
         default: return launch_nt<T, 128, ACT, PARTS>(x, Wg, Wu, p, split, stream);
     }
-}
-
-// As qg_gemm_mxfp4_rows.cu splits, whose blocks have as many bytes: one wave of two
-// CTAs per SM of 148, four blocks each at least.
-static int pick_split(int M, int tiles_n, int nk) {
-    const int64_t tiles = (int64_t)tiles_n * ceil_div(M, row_tile(M, tiles_n));
-    int split = 1;
-    while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= nk) split *= 2;
-    return split;
 }
 
 } // namespace rows
@@ -317,35 +301,36 @@ static int pick_split(int M, int tiles_n, int nk) {
 // 128x8192x4096 (unsplit) 29.9 / 30.5, 128x4096x4096 (four) 20.3 / 17.9, 256x4096x4096 (two)
 // 20.3 / 23.3, 256x1024x512 7.0 / 6.0, 256x1024x4096 17.8 / 11.0, 512x1024x4096 18.1 / 14.4,
 // 1024x1024x4096 (two) 19.5 / 21.6.
-bool use_rows(int M, int N, int K) {
+bool use_rows(int M, int N, int K, int sms) {
     const int tiles_n = ceil_div(N, rows::BW / 2);
-    return M <= 64 || rows::few_tiles(M, tiles_n) || rows::pick_split(M, tiles_n, ceil_div(K, rows::BK)) >= 4;
+    return M <= 64 || few_rows::few_tiles(M, tiles_n, sms) ||
+           few_rows::pick_split(M, tiles_n, ceil_div(K, rows::BK), sms) >= 4;
 }
 
-int rows_split_dx(int M, int N, int K) { return rows::pick_split(M, ceil_div(K, rows::BW), 2 * ceil_div(N, rows::BK)); }
+int rows_split_dx(int M, int N, int K, int sms) {
+    return few_rows::pick_split(M, ceil_div(K, rows::BW), 2 * ceil_div(N, rows::BK), sms);
+}
 
 int gated_rows(const void* X, const void* Wg, const void* Wu, void* H, void* G, void* U, bool half, int act, int M,
-               int N, int K, cudaStream_t stream) {
+               int N, int K, int sms, cudaStream_t stream) {
     const rows::Params p{M, N, K, H, G, U, nullptr};
     const void* const x[4] = {X, nullptr, nullptr, nullptr};
-    const int split = rows::pick_split(M, ceil_div(N, rows::BW / 2), ceil_div(K, rows::BK));
     const bool silu = act == QG_ACT_SILU;
     if (half)
-        return silu ? rows::launch<__half, QG_ACT_SILU, 1>(x, Wg, Wu, p, split, stream)
-                    : rows::launch<__half, QG_ACT_GELU_TANH, 1>(x, Wg, Wu, p, split, stream);
-    return silu ? rows::launch<__nv_bfloat16, QG_ACT_SILU, 1>(x, Wg, Wu, p, split, stream)
-                : rows::launch<__nv_bfloat16, QG_ACT_GELU_TANH, 1>(x, Wg, Wu, p, split, stream);
+        return silu ? rows::launch<__half, QG_ACT_SILU, 1>(x, Wg, Wu, p, sms, stream)
+                    : rows::launch<__half, QG_ACT_GELU_TANH, 1>(x, Wg, Wu, p, sms, stream);
+    return silu ? rows::launch<__nv_bfloat16, QG_ACT_SILU, 1>(x, Wg, Wu, p, sms, stream)
+                : rows::launch<__nv_bfloat16, QG_ACT_GELU_TANH, 1>(x, Wg, Wu, p, sms, stream);
 }
 
 int gated_rows_dx(const void* const (&d)[4], const void* Wg, const void* Wu, void* dX, bool half, int M, int N, int K,
-                  cudaStream_t stream) {
+                  int sms, cudaStream_t stream) {
     const rows::Params p{M, N, K, dX, nullptr, nullptr, nullptr};
-    const int split = rows_split_dx(M, N, K);
     if (d[2])
-        return half ? rows::launch<__half, rows::DX, 2>(d, Wg, Wu, p, split, stream)
-                    : rows::launch<__nv_bfloat16, rows::DX, 2>(d, Wg, Wu, p, split, stream);
-    return half ? rows::launch<__half, rows::DX, 1>(d, Wg, Wu, p, split, stream)
-                : rows::launch<__nv_bfloat16, rows::DX, 1>(d, Wg, Wu, p, split, stream);
+        return half ? rows::launch<__half, rows::DX, 2>(d, Wg, Wu, p, sms, stream)
+                    : rows::launch<__nv_bfloat16, rows::DX, 2>(d, Wg, Wu, p, sms, stream);
+    return half ? rows::launch<__half, rows::DX, 1>(d, Wg, Wu, p, sms, stream)
+                : rows::launch<__nv_bfloat16, rows::DX, 1>(d, Wg, Wu, p, sms, stream);
 }
 
 } // namespace ffn

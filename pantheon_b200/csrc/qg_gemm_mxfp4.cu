@@ -467,12 +467,6 @@ __device__ __forceinline__ void umma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc,
         : "memory");
 }
 
-// One commit that arrives on the same barrier of both CTAs of the pair.
-__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
-}
-
 template <int OUT, int ACT>
 __global__ void __launch_bounds__(P_THREADS, 1)
 gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -738,6 +732,8 @@ static int launch_gemm(const void* A, const void* B, const void* B2, GemmParams 
     DeviceInfo* info = nullptr;
     int rc = current_device_info(&info);
     if (rc) return rc;
+    if (use_rows(p.M, p.N, p.K, ACT >= 0, info->sm_count))
+        return gemm_rows(A, p.sfa, B, p.sfb, B2, p.sfb2, p.C, p.SFC, OUT, ACT, p.vec, p.M, p.N, p.K, info->sm_count, stream);
     if ((rc = device_status_ptr(&p.status))) return rc;
     CUtensorMap tmA, tmB, tmB2;
     const uint64_t row = (uint64_t)p.K / 2;
@@ -799,17 +795,14 @@ int gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, v
     if (rc) return rc;
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFB), nullptr, C, nullptr,
                      nullptr, 1, false};
-    const bool few = mx::use_rows(M, N, K, false);
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)C % 2 == 0, "qg_gemm_mxfp4: C is not aligned to its element");
             p.vec = N % 8 == 0 && ((uintptr_t)C & 15) == 0;
-            if (few) return mx::gemm_rows(A, SFA, B, SFB, nullptr, nullptr, C, nullptr, out_type, -1, p.vec, M, N, K, stream);
             return mx::launch_gemm<QG_OUT_BF16, -1>(A, B, nullptr, p, stream);
         case QG_OUT_F32:
             QG_CHECK_ARG((uintptr_t)C % 4 == 0, "qg_gemm_mxfp4: C is not aligned to its element");
             p.vec = N % 4 == 0 && ((uintptr_t)C & 15) == 0;
-            if (few) return mx::gemm_rows(A, SFA, B, SFB, nullptr, nullptr, C, nullptr, out_type, -1, p.vec, M, N, K, stream);
             return mx::launch_gemm<QG_OUT_F32, -1>(A, B, nullptr, p, stream);
         default: set_error("qg_gemm_mxfp4: out_type %d (bf16 or f32)", out_type); return QG_ERR_ARG;
     }
@@ -824,18 +817,16 @@ int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void*
     QG_CHECK_ARG(act == QG_ACT_SILU || act == QG_ACT_GELU_TANH, "qg_gemm_gated_mxfp4: unknown activation %d", act);
     mx::GemmParams p{M, N, K, static_cast<const uint8_t*>(SFA), static_cast<const uint8_t*>(SFG),
                      static_cast<const uint8_t*>(SFU), H, static_cast<uint8_t*>(SFH), nullptr, 1, false};
-    const bool silu = act == QG_ACT_SILU, few = mx::use_rows(M, N, K, true);
+    const bool silu = act == QG_ACT_SILU;
     switch (out_type) {
         case QG_OUT_BF16:
             QG_CHECK_ARG((uintptr_t)H % 2 == 0, "qg_gemm_gated_mxfp4: H is not aligned to its element");
             p.vec = N % 8 == 0 && ((uintptr_t)H & 15) == 0;
-            if (few) return mx::gemm_rows(A, SFA, Wg, SFG, Wu, SFU, H, nullptr, out_type, act, p.vec, M, N, K, stream);
             return silu ? mx::launch_gemm<QG_OUT_BF16, QG_ACT_SILU>(A, Wg, Wu, p, stream)
                         : mx::launch_gemm<QG_OUT_BF16, QG_ACT_GELU_TANH>(A, Wg, Wu, p, stream);
         case QG_OUT_F32:
             QG_CHECK_ARG((uintptr_t)H % 4 == 0, "qg_gemm_gated_mxfp4: H is not aligned to its element");
             p.vec = N % 4 == 0 && ((uintptr_t)H & 15) == 0;
-            if (few) return mx::gemm_rows(A, SFA, Wg, SFG, Wu, SFU, H, nullptr, out_type, act, p.vec, M, N, K, stream);
             return silu ? mx::launch_gemm<QG_OUT_F32, QG_ACT_SILU>(A, Wg, Wu, p, stream)
                         : mx::launch_gemm<QG_OUT_F32, QG_ACT_GELU_TANH>(A, Wg, Wu, p, stream);
         case QG_OUT_MXFP4:
@@ -843,7 +834,6 @@ int gemm_gated_mxfp4(const void* A, const void* SFA, const void* Wg, const void*
             QG_CHECK_ARG(N % 32 == 0, "qg_gemm_gated_mxfp4: N=%d must be a multiple of 32 for an MXFP4 result", N);
             QG_CHECK_ARG((((uintptr_t)H | (uintptr_t)SFH) & 15) == 0,
                          "qg_gemm_gated_mxfp4: an MXFP4 result must be 16-byte aligned");
-            if (few) return mx::gemm_rows(A, SFA, Wg, SFG, Wu, SFU, H, SFH, out_type, act, false, M, N, K, stream);
             return silu ? mx::launch_gemm<QG_OUT_MXFP4, QG_ACT_SILU>(A, Wg, Wu, p, stream)
                         : mx::launch_gemm<QG_OUT_MXFP4, QG_ACT_GELU_TANH>(A, Wg, Wu, p, stream);
         default: set_error("qg_gemm_gated_mxfp4: out_type %d (bf16, f32 or mxfp4)", out_type); return QG_ERR_ARG;

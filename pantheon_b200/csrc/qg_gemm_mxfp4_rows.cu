@@ -22,6 +22,7 @@
 //   warps 2-5   scale writers (shared memory -> TMEM), then the epilogue.
 // All barrier waits are bounded (qg_ptx.cuh).
 #include "qg_common.cuh"
+#include "qg_few_rows.cuh"
 #include "qg_formats.cuh"
 #include "qg_gated.cuh"
 #include "qg_launch.cuh"
@@ -376,35 +377,11 @@ static int launch_nt(const void* X, const void* W, const void* W2, Params p, int
     return QG_OK;
 }
 
-// Whether every tile of 64 rows gets four CTAs in one wave (two per SM of 148).
-static bool few_tiles(int M, int tiles_n) { return 4 * (int64_t)tiles_n * ceil_div(M, 64) <= 2 * 148; }
-
-// Rows of A per tile: 128 only where they are many (128 / 64 rows, us: 128x1024x4096
-// 6.4 / 5.3, 512x1024x8192 10.5 / 8.4, 512x1024x4096 6.8 / 6.9).
-static int row_tile(int M, int tiles_n) {
-    if (M <= 64) return M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    return few_tiles(M, tiles_n) ? 64 : 128;
-}
-
-// CTAs that share a tile's K.
-static int pick_split(int M, int tiles_n, int K) {
-    const int nk = (K + BK - 1) / BK;
-    const int64_t tiles = (int64_t)tiles_n * ceil_div(M, row_tile(M, tiles_n));
-    // As many CTAs as one wave holds, four K blocks each at least: a CTA's start and
-    // end cost 2-3 us, which a second wave pays again, and the join grows with the
-    // split.  Measured (one row, K=8192): N=28672 22.8 us unsplit, 26.1 in two, 31.5 in
-    // four; N=8192 14.1, 10.7, 10.4 and 13.9 in eight; N=1024 13.3, 8.6, 6.2, 5.1.
-    // 333 x 1001 x 4128 (17 blocks): 7.4 in four, 9.6 in eight.
-    int split = 1;
-    while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= nk) split *= 2;
-    return split;
-}
-
 template <int OUT, int ACT>
-static int launch(const void* X, const void* W, const void* W2, const Params& p, cudaStream_t stream) {
+static int launch(const void* X, const void* W, const void* W2, const Params& p, int sms, cudaStream_t stream) {
     const int tiles_n = ceil_div(p.N, ACT >= 0 ? BW / 2 : BW);
-    const int nt = row_tile(p.M, tiles_n), split = pick_split(p.M, tiles_n, p.K);
-    switch (nt) {
+    const int split = few_rows::pick_split(p.M, tiles_n, ceil_div(p.K, BK), sms);
+    switch (few_rows::row_tile(p.M, tiles_n, sms)) {
         case 16: return launch_nt<16, OUT, ACT>(X, W, W2, p, split, stream);
         case 32: return launch_nt<32, OUT, ACT>(X, W, W2, p, split, stream);
         case 64: return launch_nt<64, OUT, ACT>(X, W, W2, p, split, stream);
@@ -422,25 +399,26 @@ static int launch(const void* X, const void* W, const void* W2, const Params& p,
 // eight, four); 192x8192x8192 16.7 / 17.9 / 15.9, 512x4096x14336 21.4 / - / 22.4,
 // 256x4096x1024 7.1 / 5.6 / 6.5 (neither); gated 64x14336x4096 16.5 / 15.5 / 19.5,
 // 128x14336x4096 19.0 / 16.7 / 20.4.
-bool use_rows(int M, int N, int K, bool is_gated) {
+bool use_rows(int M, int N, int K, bool is_gated, int sms) {
     const int tiles_n = ceil_div(N, is_gated ? rows::BW / 2 : rows::BW);
-    return M <= (is_gated ? 32 : 64) || rows::few_tiles(M, tiles_n) || rows::pick_split(M, tiles_n, K) >= 4;
+    return M <= (is_gated ? 32 : 64) || few_rows::few_tiles(M, tiles_n, sms) ||
+           few_rows::pick_split(M, tiles_n, ceil_div(K, rows::BK), sms) >= 4;
 }
 
 int gemm_rows(const void* X, const void* SFX, const void* W, const void* SFW, const void* W2, const void* SFW2, void* C,
-              void* SFC, int out_type, int act, bool vec, int M, int N, int K, cudaStream_t stream) {
+              void* SFC, int out_type, int act, bool vec, int M, int N, int K, int sms, cudaStream_t stream) {
     const rows::Params p{M, N, K, static_cast<const uint8_t*>(SFX), static_cast<const uint8_t*>(SFW),
                          static_cast<const uint8_t*>(SFW2), C, static_cast<uint8_t*>(SFC), nullptr, vec};
     if (act < 0)
-        return out_type == QG_OUT_F32 ? rows::launch<QG_OUT_F32, -1>(X, W, W2, p, stream)
-                                      : rows::launch<QG_OUT_BF16, -1>(X, W, W2, p, stream);
+        return out_type == QG_OUT_F32 ? rows::launch<QG_OUT_F32, -1>(X, W, W2, p, sms, stream)
+                                      : rows::launch<QG_OUT_BF16, -1>(X, W, W2, p, sms, stream);
     if (act == QG_ACT_SILU)
-        return out_type == QG_OUT_F32    ? rows::launch<QG_OUT_F32, QG_ACT_SILU>(X, W, W2, p, stream)
-               : out_type == QG_OUT_BF16 ? rows::launch<QG_OUT_BF16, QG_ACT_SILU>(X, W, W2, p, stream)
-                                         : rows::launch<QG_OUT_MXFP4, QG_ACT_SILU>(X, W, W2, p, stream);
-    return out_type == QG_OUT_F32    ? rows::launch<QG_OUT_F32, QG_ACT_GELU_TANH>(X, W, W2, p, stream)
-           : out_type == QG_OUT_BF16 ? rows::launch<QG_OUT_BF16, QG_ACT_GELU_TANH>(X, W, W2, p, stream)
-                                     : rows::launch<QG_OUT_MXFP4, QG_ACT_GELU_TANH>(X, W, W2, p, stream);
+        return out_type == QG_OUT_F32    ? rows::launch<QG_OUT_F32, QG_ACT_SILU>(X, W, W2, p, sms, stream)
+               : out_type == QG_OUT_BF16 ? rows::launch<QG_OUT_BF16, QG_ACT_SILU>(X, W, W2, p, sms, stream)
+                                         : rows::launch<QG_OUT_MXFP4, QG_ACT_SILU>(X, W, W2, p, sms, stream);
+    return out_type == QG_OUT_F32    ? rows::launch<QG_OUT_F32, QG_ACT_GELU_TANH>(X, W, W2, p, sms, stream)
+           : out_type == QG_OUT_BF16 ? rows::launch<QG_OUT_BF16, QG_ACT_GELU_TANH>(X, W, W2, p, sms, stream)
+                                     : rows::launch<QG_OUT_MXFP4, QG_ACT_GELU_TANH>(X, W, W2, p, sms, stream);
 }
 
 } // namespace mx

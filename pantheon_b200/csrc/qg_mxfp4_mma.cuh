@@ -29,6 +29,13 @@ __device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// One commit that arrives on the same barrier of both CTAs of a pair (the commit of
+// this thread's products; pair `pair` of the cluster).
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar, uint32_t pair = 0) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_u32(bar)), "h"((uint16_t)(3u << (2 * pair))) : "memory");
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
