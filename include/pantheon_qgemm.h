@@ -355,10 +355,13 @@ QG_API int  qg_gemm_gated_f16(const void* X, const void* Wg, const void* Wu, voi
                               int M, int N, int K, void* stream);
 
 /* The backward pass, from dH [M,N] and what the forward pass read and kept:
- *   dG = dH * U * act'(G), dU = dH * act(G)        (rounded to the type where
- *                                                   M N > 65536)
+ *   dG = dH * U * act'(G), dU = dH * act(G)
  *   dX = dG Wg + dU Wu [M,K],  dWg = dG^T X, dWu = dU^T X [N,K]
- * fp32 accumulate, results of the operands' type (written, not added to).  dX, or
+ * fp32 accumulate, results of the operands' type (written, not added to).  dG and
+ * dU enter the products rounded to the type where M N > 65536, and as two terms, the
+ * value so rounded and the rest so rounded, up to there: accuracy and the workspace's
+ * size step at that line.  In fp16 they keep its range in either form: below 2^-25
+ * they are 0, past 65504 infinite (scale dH accordingly).  dX, or
  * dWg and dWu together, may be null: not computed.  `workspace`
  * (qg_gemm_gated_backward_workspace_bytes, 16-byte aligned, any contents) holds
  * dG and dU (with what their rounding left out, where M N <= 65536); calls that share one must not overlap on the GPU.

@@ -28,18 +28,24 @@
 // and every CTA joins a share of the columns over distributed shared memory, in
 // rank order (the same bits on every run, no workspace).
 // dG and dU are operands of the tensor cores, so rounded to the type: an error of
-// half a step in each, of the size of the result's own rounding.  Where they hold
-// few values (M N <= 65536), a handful of which can carry a sum, they go as two
-// terms (value and remainder; a stage then holds both beside one block of B) and
-// that rounding is gone; such calls last as long as their launches.  With more
-// values the second term would double the products' time.
+// half a step in each, of the size of the result's own rounding (gradients of
+// 4096x8192x4096 are off by 0.0023 of their norm in bf16, against 0.0017 from their own
+// rounding alone; fp16 0.00029 and 0.00021).  In two terms (value and remainder; a
+// stage then holds both beside one block of B) that rounding is gone, at twice the
+// products and the workspace.  The line between the two is a plain one of cost, M N
+// <= 65536, whatever the sums' lengths (M for dWg and dWu, 2 N for dX); accuracy and
+// workspace step there.  All gradients, two terms / one on the line's other side:
+// 16x4096x4096 37.0 / 37.1 us (4104), 8x8192x4096 63.0 / 60.9 (8200), 256x256x1024
+// 10.6 / 8.9 (264), 128x512x1024 15.0 / 11.1 (520), 1024x64x1024 14.7 / 10.3 (72),
+// 1x65536x1024 154 / 134 (65544); the largest, where the products are the time, would
+// take twice as long.  fp16 keeps its range in either form: what is below 2^-25 is 0.
 // G and U as kept are rounded likewise; H comes from the unrounded sums.
 // Few rows have a kernel of their own for forward and dX (use_rows, use_rows_dx,
 // qg_gemm_gated_rows.cu).
 // Bound by the tensor cores: measured at 4096x8192x4096 bf16 the forward pass takes
-// 342-349 us (1.58-1.61 PFLOP/s, 0.93-0.94 of the measured rate, tensor pipe 96 %
-// active), the backward pass 740-760 us (47 of them the stream over M x N, the rest at
-// 97 % of the tensor pipe); back to back under the power cap 410 and 893 us.
+// 342-357 us (1.54-1.61 PFLOP/s, 0.90-0.94 of the measured rate, tensor pipe 97 %
+// active), the backward pass 737-760 us (47 of them the stream over M x N, the rest at
+// 98 % of the tensor pipe); back to back under the power cap 403 and 899 us.
 // All barrier waits are bounded (qg_ptx.cuh).
 #include "qg_common.cuh"
 #include "qg_formats.cuh"

@@ -25,9 +25,10 @@
 //                scale id 0 / 2), half the scale traffic of the 16-element
 //                format.
 //   warps 6-21   epilogue: TMEM lane quarter warp % 4, and a quarter of the
-//                columns (64) each, which fit in its registers: the accumulator
-//                is free again after two tcgen05.ld per warp, and rounding,
-//                activation and stores run under the next tile's MMAs.
+//                columns (64) each, held in registers (80 a thread: fp32 results,
+//                whose rows are exchanged in twice the words, spill 12 to 56 bytes):
+//                the accumulator is free again after two tcgen05.ld per warp, and
+//                rounding, activation and stores run under the next tile's MMAs.
 // K needs to be a multiple of 32 only: the last K block loads the scale atoms
 // and issues the MMAs that K reaches; TMA fills the codes past K with zeros.
 // All barrier waits are bounded (qg_ptx.cuh).

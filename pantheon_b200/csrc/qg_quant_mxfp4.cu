@@ -43,8 +43,8 @@ struct Words {
 };
 
 // Loads a lane's words; `n` of its values exist.  Off the boundary the words reach
-// up to 14 bytes to either side, which is memory of the same tensor as long as
-// they lie in [begin, end), its first and last byte; otherwise (its corners, and
+// up to 14 bytes before them and 16 behind, between rows too; that is memory of the
+// tensor as long as they lie in [begin, end), its first and last byte; otherwise (its corners, and
 // rows that end within the lane) the values are loaded one by one, in place.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load(const T* src, int n, uintptr_t begin, uintptr_t end, Words<VEC>& v) {

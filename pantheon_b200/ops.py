@@ -380,8 +380,9 @@ def gemm_gated_bf16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor
                              U: torch.Tensor, act: int = QG_ACT_SILU, need_dx: bool = True, need_dw: bool = True,
                              workspace: torch.Tensor | None = None):
     """Gradients (dX, dWg, dWu) of gemm_gated_bf16 from dH [M,N] and the G, U it kept; a gradient
-    that is not needed is None.  Where M N > 65536, dG and dU are rounded to bf16 on the way.  `workspace` (uint8,
-    gemm_gated_backward_workspace_bytes) is allocated when not given."""
+    that is not needed is None.  dG and dU are rounded to bf16 on the way where M N > 65536, and go as
+    two terms (value and rest) up to there.  `workspace` (uint8, gemm_gated_backward_workspace_bytes)
+    is allocated when not given.  There is no autograd node: the forward call's result is detached."""
     return _gemm_gated_backward("qg_gemm_gated_bf16_backward", torch.bfloat16, dH, X, Wg, Wu, G, U, act, need_dx,
                                 need_dw, workspace)
 
@@ -389,7 +390,8 @@ def gemm_gated_bf16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor
 def gemm_gated_f16_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, G: torch.Tensor,
                             U: torch.Tensor, act: int = QG_ACT_SILU, need_dx: bool = True, need_dw: bool = True,
                             workspace: torch.Tensor | None = None):
-    """gemm_gated_bf16_backward in fp16 (values past 65504 become infinities: scale dH as usual)."""
+    """gemm_gated_bf16_backward in fp16, dG and dU too: past 65504 they are infinite, below 2^-25 zero (scale dH as
+    usual)."""
     return _gemm_gated_backward("qg_gemm_gated_f16_backward", torch.float16, dH, X, Wg, Wu, G, U, act, need_dx,
                                 need_dw, workspace)
 
